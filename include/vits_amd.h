@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define VK_ABI_VERSION 10
+#define VK_ABI_VERSION 11
 
 #define VK_OK            0
 #define VK_E_ARG        -1   /* null pointer / non-positive size / inconsistent strides */
@@ -360,6 +360,58 @@ int vk_rel_attention(const float* qkv, const float* emb_k, const float* emb_v, c
 #define VK_EXPAND_MAX_TOKENS 2048
 int vk_expand_prior(const float* durations, const float* m, const float* logs, float* m_out, float* logs_out,
                     float* frame_mask, int batch, int channels, int tokens, int frames, void* stream);
+
+/* ---- transformer blocks: attention with a bucketed relative position bias, norms around a block ----
+ * Inference and training, element type `dtype` (VK_DTYPE_F32: exact fp32 matrix instruction;
+ * VK_DTYPE_BF16: bf16 matrix inputs, fp32 accumulation and softmax).  Tensors are channel-major views
+ * [batch, channels, time] with dense time, as everywhere here; strides count elements.  Batches are
+ * padded: `*_lengths[b]` (clamped to the tensor's length; NULL: full) says how far item b goes, and
+ * nothing behind it is read.
+ *
+ * vk_bucket_attention:  q [B, heads * head_dim, queries], k, v [B, kv_heads * head_dim, keys]; head h reads
+ * kv head h / (heads / kv_heads);  pos_i = query_start[b] + i (NULL: i)
+ *     s_ij  = scale * q_i . k_j + bias[h, bucket_of[clamp(j - pos_i, +-max_distance) + max_distance]]
+ *             over j < key_lengths[b], with `causal` over j <= pos_i
+ *     lse_i = log sum_j exp(s_ij)          out_i = sum_j exp(s_ij - lse_i) v_j
+ * A query without keys, and one at or behind query_lengths[b], gets out = 0 and lse = -inf.
+ * bias [heads, buckets] fp32, bucket_of int32 [2 * max_distance + 1] (entries are clamped to the
+ * buckets); has_bias = 0: no bias.  lse [B, heads, queries] fp32, dense.  Launches with few workgroups
+ * share the keys out and join the shares through `workspace` (vk_bucket_attention_workspace_bytes; contents
+ * irrelevant before and after; calls that may overlap in time need one each).
+ *
+ * vk_bucket_attention_backward:  from q, k, v, bias, the forward's out and lse, and dout:
+ *     p = exp(s - lse), ds_ij = p_ij (dout_i . v_j - dout_i . out_i)
+ *     dq = scale ds k, dk = scale ds^T q, dv = p^T dout (summed over the heads that share a kv head),
+ *     dbias[h, c] = sum of ds_ij of head h over all pairs of bucket c (fp32)
+ * All four are written whole (zero where nothing contributes), in a fixed order of summation.        */
+#define VK_DTYPE_F32   0
+#define VK_DTYPE_BF16  1
+#define VK_BUCKET_MAX_HEAD_DIM 128
+#define VK_BUCKET_MAX_DISTANCE 1024
+#define VK_BUCKET_MAX_LENGTH   (1 << 28)
+typedef struct {
+    const void* q;     int64_t q_bstride;    int64_t q_cstride;
+    const void* k;     int64_t k_bstride;    int64_t k_cstride;
+    const void* v;     int64_t v_bstride;    int64_t v_cstride;
+    void* out;         int64_t out_bstride;  int64_t out_cstride;   /* written by the forward, read by the backward */
+    float* lse;                                                     /* likewise */
+    const void* dout;  int64_t dout_bstride; int64_t dout_cstride;  /* backward only, down to dbias */
+    void* dq;          int64_t dq_bstride;   int64_t dq_cstride;
+    void* dk;          int64_t dk_bstride;   int64_t dk_cstride;
+    void* dv;          int64_t dv_bstride;   int64_t dv_cstride;
+    float* dbias;                                                   /* [heads, buckets] dense */
+    const float* bias; const int32_t* bucket_of;
+    const int64_t* key_lengths; const int64_t* query_lengths; const int64_t* query_start;   /* [B] or NULL */
+    void* workspace;   int64_t workspace_bytes;
+    int32_t batch, heads, kv_heads, head_dim, queries, keys;
+    int32_t has_bias, buckets, max_distance, causal, dtype;
+    float   scale;
+} vk_bucket_attention_args;
+
+int64_t vk_bucket_attention_workspace_bytes(const vk_bucket_attention_args* a);
+int vk_bucket_attention(const vk_bucket_attention_args* a, void* stream);
+int64_t vk_bucket_attention_backward_workspace_bytes(const vk_bucket_attention_args* a);
+int vk_bucket_attention_backward(const vk_bucket_attention_args* a, void* stream);
 
 /* out[b, o] = bias[o] + sum_i W[o, i] * g[b, i]   (speaker-conditioning 1x1 convs on
  * [B, G, 1] inputs: decoder.py:91,112 `cond`; wn.py:41-42,66 `condition_layer`).

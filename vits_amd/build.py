@@ -19,7 +19,10 @@ LIB = os.path.join(LIBDIR, "libvits_amd.so")
 DIAG_LIB = os.path.join(LIBDIR, "libvits_amd_diag.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
-FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function"]
+# no packed fp32 instructions: some of their forms have given wrong results on this part (the host pass does
+# not know the feature and says so)
+FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def csrc_hash() -> str:

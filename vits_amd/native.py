@@ -135,6 +135,34 @@ class DdsArgs(C.Structure):
 DDS_CHANNELS = 192
 
 
+class BucketAttentionArgs(C.Structure):
+    """Mirror of ``vk_bucket_attention_args``."""
+    _fields_ = [
+        ("q", _fp), ("q_bstride", C.c_int64), ("q_cstride", C.c_int64),
+        ("k", _fp), ("k_bstride", C.c_int64), ("k_cstride", C.c_int64),
+        ("v", _fp), ("v_bstride", C.c_int64), ("v_cstride", C.c_int64),
+        ("out", _fp), ("out_bstride", C.c_int64), ("out_cstride", C.c_int64),
+        ("lse", _fp),
+        ("dout", _fp), ("dout_bstride", C.c_int64), ("dout_cstride", C.c_int64),
+        ("dq", _fp), ("dq_bstride", C.c_int64), ("dq_cstride", C.c_int64),
+        ("dk", _fp), ("dk_bstride", C.c_int64), ("dk_cstride", C.c_int64),
+        ("dv", _fp), ("dv_bstride", C.c_int64), ("dv_cstride", C.c_int64),
+        ("dbias", _fp),
+        ("bias", _fp), ("bucket_of", _fp),
+        ("key_lengths", _fp), ("query_lengths", _fp), ("query_start", _fp),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("batch", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("queries", C.c_int32), ("keys", C.c_int32),
+        ("has_bias", C.c_int32), ("buckets", C.c_int32), ("max_distance", C.c_int32), ("causal", C.c_int32),
+        ("dtype", C.c_int32), ("scale", C.c_float),
+    ]
+
+
+DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+BUCKET_MAX_HEAD_DIM, BUCKET_MAX_DISTANCE, BUCKET_MAX_LENGTH = 128, 1024, 1 << 28
+
+
 class NativeError(RuntimeError):
     pass
 
@@ -185,13 +213,17 @@ def lib():
         L.vk_dds_workspace_bytes.restype = C.c_int64
         L.vk_dds_condition.argtypes = [C.POINTER(DdsArgs), C.c_void_p]
         L.vk_dds_coupling.argtypes = [C.POINTER(DdsArgs), C.c_void_p]
+        for name in ("vk_bucket_attention", "vk_bucket_attention_backward"):
+            getattr(L, name).argtypes = [C.POINTER(BucketAttentionArgs), C.c_void_p]
+            getattr(L, name + "_workspace_bytes").argtypes = [C.POINTER(BucketAttentionArgs)]
+            getattr(L, name + "_workspace_bytes").restype = C.c_int64
         L.vk_sizeof_args.argtypes = [C.c_int]
         L.vk_sizeof_args.restype = C.c_size_t
         want = header_abi_version()
         if L.vk_abi_version() != want:
             raise NativeError(f"{_lib_path}: ABI version {L.vk_abi_version()}, include/vits_amd.h declares {want}; "
                               "rebuild with `python -m vits_amd.build`")
-        for which, mirror in enumerate((ConvArgs, PairArgs, WnArgs, TileInfo, MrfArgs, DdsArgs)):
+        for which, mirror in enumerate((ConvArgs, PairArgs, WnArgs, TileInfo, MrfArgs, DdsArgs, BucketAttentionArgs)):
             if L.vk_sizeof_args(which) != C.sizeof(mirror):
                 raise NativeError(f"{mirror.__name__} is {C.sizeof(mirror)} bytes here, "
                                   f"{L.vk_sizeof_args(which)} in the library: native.py is out of step with the header")
@@ -633,6 +665,77 @@ def rel_attention(qkv, emb_k, emb_v, mask, out, *, heads, window):
                  lambda: L.vk_rel_attention(qkv.data_ptr(), emb_k.data_ptr(), emb_v.data_ptr(), mask.data_ptr(),
                                             out.data_ptr(), B, heads, head_dim, window, T, sp), f"B{B} T{T}"),
           "vk_rel_attention")
+
+
+def _on_device(device, launch):
+    """Run ``launch`` with ``device`` current (a launch goes to the current device's context)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return launch()
+    with torch.cuda.device(device):
+        return launch()
+
+
+def _bucket_args(q, k, v, out, lse, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
+    a = BucketAttentionArgs()
+    a.q, a.q_bstride, a.q_cstride = q.data_ptr(), q.stride(0), q.stride(1)
+    a.k, a.k_bstride, a.k_cstride = k.data_ptr(), k.stride(0), k.stride(1)
+    a.v, a.v_bstride, a.v_cstride = v.data_ptr(), v.stride(0), v.stride(1)
+    a.out, a.out_bstride, a.out_cstride = out.data_ptr(), out.stride(0), out.stride(1)
+    a.lse = lse.data_ptr()
+    if bias is not None:
+        a.bias, a.bucket_of = bias.data_ptr(), bucket_of.data_ptr()
+        a.has_bias, a.buckets, a.max_distance = 1, bias.shape[1], (bucket_of.shape[0] - 1) // 2
+    if key_lengths is not None:
+        a.key_lengths = key_lengths.data_ptr()
+    if query_lengths is not None:
+        a.query_lengths = query_lengths.data_ptr()
+    if query_start is not None:
+        a.query_start = query_start.data_ptr()
+    a.batch, a.heads, a.kv_heads, a.head_dim = q.shape[0], heads, kv_heads, q.shape[1] // heads
+    a.queries, a.keys = q.shape[2], k.shape[2]
+    a.causal, a.dtype, a.scale = int(causal), DTYPES[q.dtype], scale
+    return a
+
+
+def _bucket_run(name, a, device, family_flops, nbytes):
+    """Size the workspace (stream-ordered, from torch's allocator: a graph keeps its own) and launch."""
+    L = lib()
+
+    def launch():
+        need = getattr(L, name + "_workspace_bytes")(C.byref(a))
+        check(min(need, 0), name)
+        ws = torch.empty(need, device=device, dtype=torch.uint8) if need else None
+        a.workspace, a.workspace_bytes = (ws.data_ptr() if need else None), need
+        sp = stream_ptr(device)
+        check(_timed(name[3:], family_flops, nbytes, device, lambda: getattr(L, name)(C.byref(a), sp),
+                     f"B{a.batch} H{a.heads}/{a.kv_heads} D{a.head_dim} Tq{a.queries} Tk{a.keys}"), name)
+
+    _on_device(device, launch)
+
+
+def bucket_attention(q, k, v, out, lse, bias=None, bucket_of=None, *, heads, kv_heads, key_lengths=None,
+                     query_lengths=None, query_start=None, causal=False, scale):
+    """out, lse = attention of q over k, v with a bucketed relative position bias (``vk_bucket_attention``).
+    Views [B, channels, T] with dense time; ``vits_amd.attention`` checks and allocates."""
+    assert q.is_cuda, "the HIP path needs device tensors"
+    a = _bucket_args(q, k, v, out, lse, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale)
+    _bucket_run("vk_bucket_attention", a, q.device, 4.0 * q.shape[0] * q.shape[1] * q.shape[2] * k.shape[2],
+                q.element_size() * (q.numel() + k.numel() + v.numel() + out.numel()))
+
+
+def bucket_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, bias=None, bucket_of=None, dbias=None, *, heads, kv_heads,
+                              key_lengths=None, query_lengths=None, query_start=None, causal=False, scale):
+    """dq, dk, dv (and dbias) of ``bucket_attention`` (``vk_bucket_attention_backward``)."""
+    assert q.is_cuda, "the HIP path needs device tensors"
+    a = _bucket_args(q, k, v, out, lse, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale)
+    a.dout, a.dout_bstride, a.dout_cstride = dout.data_ptr(), dout.stride(0), dout.stride(1)
+    a.dq, a.dq_bstride, a.dq_cstride = dq.data_ptr(), dq.stride(0), dq.stride(1)
+    a.dk, a.dk_bstride, a.dk_cstride = dk.data_ptr(), dk.stride(0), dk.stride(1)
+    a.dv, a.dv_bstride, a.dv_cstride = dv.data_ptr(), dv.stride(0), dv.stride(1)
+    if bias is not None:
+        a.dbias = dbias.data_ptr()
+    _bucket_run("vk_bucket_attention_backward", a, q.device, 10.0 * q.shape[0] * q.shape[1] * q.shape[2] * k.shape[2],
+                2 * q.element_size() * (q.numel() + k.numel() + v.numel() + out.numel()))
 
 
 EXPAND_MAX_TOKENS = 2048
