@@ -413,6 +413,46 @@ int vk_bucket_attention(const vk_bucket_attention_args* a, void* stream);
 int64_t vk_bucket_attention_backward_workspace_bytes(const vk_bucket_attention_args* a);
 int vk_bucket_attention_backward(const vk_bucket_attention_args* a, void* stream);
 
+/* vk_block_norm: the norms around a transformer block with its gate, residual scale and residual sum between:
+ *     z = N(y) * w_post + b_post   (w_post NULL: z = y)
+ *     h = x + scale * gate * z     (y NULL: h = x; gate, scale NULL: 1)
+ *     n = N(h) * w_pre + b_pre
+ * N over the channels of each column (b, t): VK_NORM_LAYER (v - mean) / sqrt(var + eps), VK_NORM_RMS
+ * v / sqrt(mean of squares + eps); statistics and parameters fp32, x, y, gate, h, n of type `dtype`.  n is taken of h
+ * before h is rounded for storage.  gate: [B, C, T], or with gate_per_item one value per item and channel
+ * (strides gate_bstride, gate_cstride).  Columns at or behind lengths[b] (NULL: none) are not read and written as 0.
+ * h or n may be NULL (not wanted).  channels <= VK_BLOCK_NORM_MAX_CHANNELS, eps > 0.  Outputs must not overlap inputs.
+ *
+ * vk_block_norm_backward: dh, dn (either may be NULL: zero) -> dx, dy, dgate and the parameters' gradients (each may
+ * be NULL if not wanted, but dx and, with y, dy), from h as stored, y, gate and the parameters:
+ *     g = dh + N'(dn * w_pre)   dx = g   dgate = g * scale * z   dscale = sum g * gate * z   dy = N'(g * scale * gate * w_post)
+ * The sums over columns are taken per workgroup and then over the workgroups in a fixed order, through `workspace`.  */
+#define VK_NORM_LAYER 0
+#define VK_NORM_RMS   1
+#define VK_BLOCK_NORM_MAX_CHANNELS 4096
+typedef struct {
+    const void* x;     int64_t x_bstride;     int64_t x_cstride;      /* forward only */
+    const void* y;     int64_t y_bstride;     int64_t y_cstride;
+    const void* gate;  int64_t gate_bstride;  int64_t gate_cstride;
+    const float* scale; const float* w_post; const float* b_post; const float* w_pre; const float* b_pre;   /* [C] */
+    void* h;           int64_t h_bstride;     int64_t h_cstride;      /* written by the forward, read by the backward */
+    void* n;           int64_t n_bstride;     int64_t n_cstride;      /* forward only */
+    const int64_t* lengths;
+    const void* dh;    int64_t dh_bstride;    int64_t dh_cstride;     /* backward only, down to the workspace */
+    const void* dn;    int64_t dn_bstride;    int64_t dn_cstride;
+    void* dx;          int64_t dx_bstride;    int64_t dx_cstride;
+    void* dy;          int64_t dy_bstride;    int64_t dy_cstride;
+    void* dgate;       int64_t dgate_bstride; int64_t dgate_cstride;
+    float* dscale; float* dw_post; float* db_post; float* dw_pre; float* db_pre;
+    void* workspace;   int64_t workspace_bytes;
+    int32_t batch, channels, length, gate_per_item, norm, dtype;
+    float   eps;
+} vk_block_norm_args;
+
+int vk_block_norm(const vk_block_norm_args* a, void* stream);
+int64_t vk_block_norm_backward_workspace_bytes(const vk_block_norm_args* a);
+int vk_block_norm_backward(const vk_block_norm_args* a, void* stream);
+
 /* out[b, o] = bias[o] + sum_i W[o, i] * g[b, i]   (speaker-conditioning 1x1 convs on
  * [B, G, 1] inputs: decoder.py:91,112 `cond`; wn.py:41-42,66 `condition_layer`).
  * W is [n_out, n_in] row-major (weight norm already folded). One wavefront per output. */

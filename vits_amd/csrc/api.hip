@@ -48,6 +48,7 @@ extern "C" size_t vk_sizeof_args(int which)
     case 4: return sizeof(vk_mrf_args);
     case 5: return sizeof(vk_dds_args);
     case 6: return sizeof(vk_bucket_attention_args);
+    case 7: return sizeof(vk_block_norm_args);
     default: return 0;
     }
 }

@@ -158,6 +158,30 @@ class BucketAttentionArgs(C.Structure):
     ]
 
 
+class BlockNormArgs(C.Structure):
+    """Mirror of ``vk_block_norm_args``."""
+    _fields_ = [
+        ("x", _fp), ("x_bstride", C.c_int64), ("x_cstride", C.c_int64),
+        ("y", _fp), ("y_bstride", C.c_int64), ("y_cstride", C.c_int64),
+        ("gate", _fp), ("gate_bstride", C.c_int64), ("gate_cstride", C.c_int64),
+        ("scale", _fp), ("w_post", _fp), ("b_post", _fp), ("w_pre", _fp), ("b_pre", _fp),
+        ("h", _fp), ("h_bstride", C.c_int64), ("h_cstride", C.c_int64),
+        ("n", _fp), ("n_bstride", C.c_int64), ("n_cstride", C.c_int64),
+        ("lengths", _fp),
+        ("dh", _fp), ("dh_bstride", C.c_int64), ("dh_cstride", C.c_int64),
+        ("dn", _fp), ("dn_bstride", C.c_int64), ("dn_cstride", C.c_int64),
+        ("dx", _fp), ("dx_bstride", C.c_int64), ("dx_cstride", C.c_int64),
+        ("dy", _fp), ("dy_bstride", C.c_int64), ("dy_cstride", C.c_int64),
+        ("dgate", _fp), ("dgate_bstride", C.c_int64), ("dgate_cstride", C.c_int64),
+        ("dscale", _fp), ("dw_post", _fp), ("db_post", _fp), ("dw_pre", _fp), ("db_pre", _fp),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("batch", C.c_int32), ("channels", C.c_int32), ("length", C.c_int32), ("gate_per_item", C.c_int32),
+        ("norm", C.c_int32), ("dtype", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+NORM_LAYER, NORM_RMS = 0, 1
+BLOCK_NORM_MAX_CHANNELS = 4096
 DTYPE_F32, DTYPE_BF16 = 0, 1
 DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 BUCKET_MAX_HEAD_DIM, BUCKET_MAX_DISTANCE, BUCKET_MAX_LENGTH = 128, 1024, 1 << 28
@@ -217,13 +241,17 @@ def lib():
             getattr(L, name).argtypes = [C.POINTER(BucketAttentionArgs), C.c_void_p]
             getattr(L, name + "_workspace_bytes").argtypes = [C.POINTER(BucketAttentionArgs)]
             getattr(L, name + "_workspace_bytes").restype = C.c_int64
+        L.vk_block_norm.argtypes = L.vk_block_norm_backward.argtypes = [C.POINTER(BlockNormArgs), C.c_void_p]
+        L.vk_block_norm_backward_workspace_bytes.argtypes = [C.POINTER(BlockNormArgs)]
+        L.vk_block_norm_backward_workspace_bytes.restype = C.c_int64
         L.vk_sizeof_args.argtypes = [C.c_int]
         L.vk_sizeof_args.restype = C.c_size_t
         want = header_abi_version()
         if L.vk_abi_version() != want:
             raise NativeError(f"{_lib_path}: ABI version {L.vk_abi_version()}, include/vits_amd.h declares {want}; "
                               "rebuild with `python -m vits_amd.build`")
-        for which, mirror in enumerate((ConvArgs, PairArgs, WnArgs, TileInfo, MrfArgs, DdsArgs, BucketAttentionArgs)):
+        for which, mirror in enumerate((ConvArgs, PairArgs, WnArgs, TileInfo, MrfArgs, DdsArgs, BucketAttentionArgs,
+                                        BlockNormArgs)):
             if L.vk_sizeof_args(which) != C.sizeof(mirror):
                 raise NativeError(f"{mirror.__name__} is {C.sizeof(mirror)} bytes here, "
                                   f"{L.vk_sizeof_args(which)} in the library: native.py is out of step with the header")
@@ -736,6 +764,61 @@ def bucket_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, bias=None, bu
         a.dbias = dbias.data_ptr()
     _bucket_run("vk_bucket_attention_backward", a, q.device, 10.0 * q.shape[0] * q.shape[1] * q.shape[2] * k.shape[2],
                 2 * q.element_size() * (q.numel() + k.numel() + v.numel() + out.numel()))
+
+
+def _block_norm_args(like, gate, scale, post, pre, norm, eps, lengths, **views):
+    a = BlockNormArgs()
+    for name, t in views.items():
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+            setattr(a, name + "_bstride", t.stride(0))
+            setattr(a, name + "_cstride", t.stride(1))
+    a.batch, a.channels, a.length = like.shape
+    if gate is not None:
+        a.gate, a.gate_bstride, a.gate_cstride = gate.data_ptr(), gate.stride(0), gate.stride(1)
+        a.gate_per_item = int(gate.shape[2] == 1 and like.shape[2] != 1)
+    for name, t in (("scale", scale), ("w_post", post and post[0]), ("b_post", post and post[1]), ("w_pre", pre and pre[0]),
+                    ("b_pre", pre and pre[1]), ("lengths", lengths)):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    a.norm, a.dtype, a.eps = norm, DTYPES[like.dtype], eps
+    return a
+
+
+def block_norm(x, y, h, n, *, gate=None, scale=None, post=None, pre=None, norm=NORM_LAYER, eps=1e-5, lengths=None):
+    """h = x + scale * gate * norm(y), n = norm(h) in one launch (``vk_block_norm``); y, h, n may be None.  ``post``, ``pre``:
+    (weight, bias or None) or None.  ``vits_amd.block_norm`` checks and allocates."""
+    assert x.is_cuda, "the HIP path needs device tensors"
+    a = _block_norm_args(x, gate, scale, post, pre, norm, eps, lengths, x=x, y=y, h=h, n=n)
+    nbytes = x.element_size() * sum(t.numel() for t in (x, y, h, n, gate) if t is not None)
+    L = lib()
+    _on_device(x.device, lambda: check(
+        _timed("block_norm", 20.0 * x.numel(), nbytes, x.device, lambda: L.vk_block_norm(C.byref(a), stream_ptr(x.device)),
+               f"B{a.batch} C{a.channels} T{a.length}"), "vk_block_norm"))
+
+
+def block_norm_backward(dh, dn, h, y, dx, dy, *, gate=None, dgate=None, scale=None, dscale=None, post=None, dpost=None, pre=None,
+                        dpre=None, norm=NORM_LAYER, eps=1e-5, lengths=None):
+    """The gradients of ``block_norm`` (``vk_block_norm_backward``); ``dpost``, ``dpre`` like ``post``, ``pre``."""
+    assert dx.is_cuda, "the HIP path needs device tensors"
+    a = _block_norm_args(dx, gate, scale, post, pre, norm, eps, lengths, y=y, h=h, dh=dh, dn=dn, dx=dx, dy=dy, dgate=dgate)
+    for name, t in (("dscale", dscale), ("dw_post", dpost and dpost[0]), ("db_post", dpost and dpost[1]),
+                    ("dw_pre", dpre and dpre[0]), ("db_pre", dpre and dpre[1])):
+        if t is not None:
+            setattr(a, name, t.data_ptr())
+    nbytes = dx.element_size() * sum(t.numel() for t in (dh, dn, h, y, gate, dx, dy, dgate) if t is not None)
+    L = lib()
+
+    def launch():
+        need = L.vk_block_norm_backward_workspace_bytes(C.byref(a))
+        check(min(need, 0), "vk_block_norm_backward")
+        ws = torch.empty(need, device=dx.device, dtype=torch.uint8) if need else None
+        a.workspace, a.workspace_bytes = (ws.data_ptr() if need else None), need
+        check(_timed("block_norm_backward", 40.0 * dx.numel(), nbytes, dx.device,
+                     lambda: L.vk_block_norm_backward(C.byref(a), stream_ptr(dx.device)),
+                     f"B{a.batch} C{a.channels} T{a.length}"), "vk_block_norm_backward")
+
+    _on_device(dx.device, launch)
 
 
 EXPAND_MAX_TOKENS = 2048
