@@ -17,8 +17,6 @@ captured with the stream of that pass.  A training step that is captured calls `
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import native
@@ -114,8 +112,8 @@ def _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, 
             raise ValueError(f"bias must be a contiguous float32 [{heads}, {buckets.num_buckets}] on {q.device}")
         table = buckets.table(q.device)
     scale = (C // heads) ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not 0 < scale < 1e30:
+        raise ValueError("scale must be positive and finite")
     return kv_heads, scale, table
 
 

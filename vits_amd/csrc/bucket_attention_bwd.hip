@@ -10,16 +10,34 @@
 namespace {
 using namespace vkba;
 
+// Waves per SIMD a kernel is built for, positions of a staged tile, 32-position blocks taken in one step.  Up to 96
+// channels (fp32: 64) two waves fit a SIMD's registers and one computes while the other waits; wider heads run one
+// wave with two blocks in one step instead.
+template <typename T, int DP, int KW>
+struct Shape {
+    static constexpr bool WIDE = sizeof(T) == 2 ? DP > 96 : DP > 64;
+    static constexpr int MIN_WAVES = WIDE ? 1 : 2;
+#ifndef WKT
+#define WKT 64
+#endif
+    static constexpr int KT = WIDE && sizeof(T) == 2 && KW == 2 ? WKT : 64;
+    static constexpr int NS = KT / 32 / KW, SP = WIDE ? NS : 1;
+};
+
 constexpr int DGP = 33;         // pitch of a wave's 32 x 32 block of logit gradients
 
 // dq_i = scale * sum_j ds_ij k_j, and the sums of ds over the diagonals j - pos_i = const (the bias
 // gradient by offset).  Scores are transposed as in the forward pass: a query is a lane.
-template <typename T, int DP>
-__global__ __launch_bounds__(NTHR)
+//
+// KW = 2: half of the waves take the first, half the second 32 keys of every tile (64 queries per workgroup
+// instead of 128) and their sums are joined through LDS at the end.
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(NTHR, (Shape<T, DP, KW>::MIN_WAVES))
 void bucket_dq_kernel(Dev p)
 {
     using F = typename Num<T>::frag;
-    constexpr int KS = Num<T>::KS, PT = Num<T>::PT, QT = NWAVE * 32;
+    using S = Shape<T, DP, KW>;
+    constexpr int KT = S::KT, NS = S::NS, SP = S::SP, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, QW = NWAVE / KW, QT = QW * 32;
     extern __shared__ __align__(16) unsigned char lds[];
     T* ki = reinterpret_cast<T*>(lds);
     T* vi = ki + DP * PT;
@@ -29,58 +47,60 @@ void bucket_dq_kernel(Dev p)
     float* hist = tab + ((offsets + 3) & ~3) + wave * offsets;                  // this wave's diagonal sums
     float* blk_ds = tab + ((offsets + 3) & ~3) + NWAVE * offsets + wave * 32 * DGP;
 
-    int unit, within;
-    if (!place(p, unit, within)) return;
-    const int kvh = unit % (p.heads / p.group), b = unit / (p.heads / p.group);
-    const int head = kvh * p.group + within % p.group;
-    const int qt = p.tiles - 1 - within / p.group;
+    const Place at = place(p);
+    if (!at.any) return;
+    const int b = at.b, kvh = at.kvh, head = kvh * p.group + at.within % p.group;
+    const int qt = p.tiles - 1 - at.within / p.group;
     const Item it = item_of(p, b);
-    const int q0 = qt * QT + wave * 32, qi = q0 + (l & 31);
+    const int qw = wave / KW, kw = wave % KW;
+    const int q0 = qt * QT + qw * 32, qi = q0 + (l & 31);
     const bool valid = qi < it.nq;
     const int64_t row = ((int64_t)b * p.heads + head) * p.queries + qi;
     const int64_t hd = (int64_t)head * p.head_dim;
 
     const T* kg = (const T*)p.k + (int64_t)b * p.kb + (int64_t)kvh * p.head_dim * p.kc;
     const T* vg = (const T*)p.v + (int64_t)b * p.vb + (int64_t)kvh * p.head_dim * p.vc;
-    F qf[1][DP / KS], dof[1][DP / KS];
-    load_frags<DP>(qf[0], (const T*)p.q + (int64_t)b * p.qb + hd * p.qc + qi, p.qc, p.head_dim, valid);
-    load_frags<DP>(dof[0], (const T*)p.dout + (int64_t)b * p.dob + hd * p.doc + qi, p.doc, p.head_dim, valid);
-    // delta enters every logit gradient of its row with the same sign, so its error adds up coherently in the
-    // bias gradient: summed in 64 bits, rounded once
-    double delta64 = 0.0;
-    if (valid) {
-        const T* og = (const T*)p.o + (int64_t)b * p.ob + hd * p.oc + qi;
-        const T* dg = (const T*)p.dout + (int64_t)b * p.dob + hd * p.doc + qi;
-        for (int d = h; d < p.head_dim; d += 2) delta64 = fma((double)(float)og[(int64_t)d * p.oc], (double)(float)dg[(int64_t)d * p.doc], delta64);
-    }
-    delta64 += __shfl_xor(delta64, 32);
-    const float delta = (float)delta64;
-    float lse2 = __builtin_inff();
-    if (valid) {
-        const float v = p.lse_in[row];
-        lse2 = v == -__builtin_inff() ? __builtin_inff() : v * LOG2E;          // no keys: all probabilities 0
-        if (h == 0) p.delta[row] = delta;
-    }
-    stage_bias(tab, p, head);
-    if (p.bias) for (int o = l; o < offsets; o += 64) hist[o] = 0.0f;
-
+    // keys this workgroup walks over
     int end = it.nk;
     const int last_q = min(qt * QT + QT, it.nq) - 1;
     if (p.causal) end = clampi(it.start + last_q + 1, 0, end);
     if (qt * QT >= it.nq) end = 0;
 
-    f32x16 acc[1][DP / 32];
+    Tile<T, DP, KT> kt, vt;
+    F qf[DP / KS], dof[DP / KS];
+    // delta enters every logit gradient of its row with the same sign, so its error adds up coherently in the
+    // bias gradient: summed in 64 bits, rounded once
+    float delta = 0.0f;
+    if (qt * QT < it.nq) {
+        OwnRows<T, DP, KT, QW> rq, rd;
+        rq.load((const T*)p.o + (int64_t)b * p.ob + hd * p.oc, p.oc, p.head_dim, qt * QT, it.nq);
+        rd.load((const T*)p.dout + (int64_t)b * p.dob + hd * p.doc, p.doc, p.head_dim, qt * QT, it.nq);
+        rq.frags(qf, ki, vi, qw);
+        rq.load((const T*)p.q + (int64_t)b * p.qb + hd * p.qc, p.qc, p.head_dim, qt * QT, it.nq);
+        rd.frags(dof, ki, vi, qw);
+        delta = (float)dot_frags(qf, dof);
+        if (end > 0) {
+            kt.load(kg, p.kc, p.head_dim, 0, end);
+            vt.load(vg, p.vc, p.head_dim, 0, end);
+        }
+        rq.frags(qf, ki, vi, qw);
+    }
+    float lse2 = __builtin_inff();
+    if (valid) {
+        const float v = p.lse_in[row];
+        lse2 = v == -__builtin_inff() ? __builtin_inff() : v * LOG2E;          // no keys: all probabilities 0
+        if (h == 0 && kw == 0) p.delta[row] = delta;
+    }
+    stage_bias(tab, p, head);
+    if (p.bias) for (int o = l; o < offsets; o += 64) hist[o] = 0.0f;
+
+    f32x16 acc[DP / 32];
 #pragma unroll
     for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[0][blk][r] = 0.0f;
-    float far_left = 0.0f, far_right = 0.0f;
+        for (int r = 0; r < 16; ++r) acc[blk][r] = 0.0f;
+    double far_left = 0.0, far_right = 0.0;
 
-    Tile<T, DP> kt, vt;
-    if (end > 0) {
-        kt.load(kg, p.kc, p.head_dim, 0, end);
-        vt.load(vg, p.vc, p.head_dim, 0, end);
-    }
     const int pos0 = it.start + q0, pos = pos0 + (l & 31);
     for (int j0 = 0; j0 < end; j0 += KT) {
         __syncthreads();
@@ -92,47 +112,51 @@ void bucket_dq_kernel(Dev p)
             vt.load(vg, p.vc, p.head_dim, j0 + KT, end);
         }
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            const int js = j0 + 32 * sub;
+        for (int step = 0; step < NS / SP; ++step) {
+            const int c0 = 32 * (kw * NS + step * SP), js = j0 + c0;            // this step's keys: SP * 32 from here
             if (js >= end || (p.causal && js > pos0 + 31)) continue;
-            f32x16 s[1], dp[1];
+            const int lo = js - (pos0 + 31), hi = js + 32 * SP - 1 - pos0, side = bias_side(p, lo, hi);
+            f32x16 s[SP], dp[SP];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { s[0][r] = 0.0f; dp[0][r] = -delta; }
-            dot_channels<DP, 1>(s, ki, 32 * sub, qf);
-            dot_channels<DP, 1>(dp, vi, 32 * sub, dof);
-            const int lo = js - (pos0 + 31), hi = js + 31 - pos0;
-            const BlockBias bb = block_bias(tab, p, lo, hi);
-            if (bb.near_) {
+            for (int i = 0; i < SP; ++i) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int off = clampi(js + acc_row(r, h) - pos, -p.far_, p.far_);
-                    s[0][r] = fmaf(s[0][r], p.c, tab[off + p.far_] - lse2);
-                }
+                for (int r = 0; r < 16; ++r) { s[i][r] = 0.0f; dp[i][r] = -delta; }
+                dot_channels<DP, PT>(s[i], ki, c0 + 32 * i, qf);
+                dot_channels<DP, PT>(dp[i], vi, c0 + 32 * i, dof);
+            }
+            if (side != BIAS_NEAR && js + 32 * SP <= end && !(p.causal && hi > 0)) {
+                const float shift = bias_flat(tab, p, side) - lse2;
+#pragma unroll
+                for (int i = 0; i < SP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dp[i][r] *= exp2_hw(fmaf(s[i][r], p.c, shift));
             } else {
+                const int stop = (p.causal ? min(end, pos + 1) : end) - js;
+                const float flat = bias_flat(tab, p, side);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], p.c, bb.flat - lse2);
+                for (int i = 0; i < SP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = 32 * i + acc_row(r, h);
+                        const float bias = side == BIAS_NEAR ? tab[clampi(js + row - pos, -p.far_, p.far_) + p.far_] : flat;
+                        dp[i][r] *= exp2_hw(fmaf(s[i][r], p.c, bias - lse2));
+                        if (row >= stop) dp[i][r] = 0.0f;
+                    }
             }
+            if (side == BIAS_NEAR) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) dp[0][r] *= exp2_hw(s[0][r]);
-            if (js + 32 > end || (p.causal && hi > 0)) {
-                const int stop = p.causal ? min(end, pos + 1) : end;
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (js + acc_row(r, h) >= stop) dp[0][r] = 0.0f;
-            }
-            if (p.bias) {
-                if (bb.near_) {
+                for (int i = 0; i < SP; ++i) {
                     // transposed through LDS so that a lane owns one diagonal of the block
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) blk_ds[acc_row(r, h) * DGP + (l & 31)] = dp[0][r];
+                    for (int r = 0; r < 16; ++r) blk_ds[acc_row(r, h) * DGP + (l & 31)] = dp[i][r];
                     wave_lds_fence();
                     const int dg = l - 31;                      // key index - query index
                     float sum = 0.0f;
                     if (l < 63) {
                         const int i0 = dg < 0 ? -dg : 0, i1 = dg > 0 ? 32 - dg : 32;
-                        for (int i = i0; i < i1; ++i) sum += blk_ds[(i + dg) * DGP + i];
+                        for (int e = i0; e < i1; ++e) sum += blk_ds[(e + dg) * DGP + e];
                     }
-                    const int off = js - pos0 + dg;
+                    const int off = js + 32 * i - pos0 + dg;
                     // offsets beyond the table all fall on its ends: those lanes keep their sum to themselves
                     if (l < 63) {
                         if (off <= -p.far_) far_left += sum;
@@ -140,32 +164,50 @@ void bucket_dq_kernel(Dev p)
                         else hist[off + p.far_] += sum;
                     }
                     wave_lds_fence();
-                } else {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += dp[0][r];
-                    if (hi <= -p.far_) far_left += sum; else far_right += sum;
                 }
+            } else if (side != BIAS_NONE) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < SP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sum += dp[i][r];
+                if (side == BIAS_LEFT) far_left += sum; else far_right += sum;
             }
-            dot_positions<DP, 1>(acc, ki, 32 * sub, dp);
+#pragma unroll
+            for (int i = 0; i < SP; ++i) dot_positions<DP, PT>(acc, ki, c0 + 32 * i, dp[i]);
         }
     }
 
-    if (qi < p.queries) {
+    if constexpr (KW == 2) {
+        __syncthreads();                                    // the images are free
+        float* red = reinterpret_cast<float*>(lds) + qw * DP * 32 + (l & 31);
+        if (kw == 1)
+#pragma unroll
+            for (int blk = 0; blk < DP / 32; ++blk)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) red[(32 * blk + acc_row(r, h)) * 32] = acc[blk][r];
+        __syncthreads();
+        if (kw == 0)
+#pragma unroll
+            for (int blk = 0; blk < DP / 32; ++blk)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[blk][r] += red[(32 * blk + acc_row(r, h)) * 32];
+    }
+    if (qi < p.queries && kw == 0) {
         T* dqg = (T*)p.dq + (int64_t)b * p.dqb + hd * p.dqc + qi;
 #pragma unroll
         for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * blk + acc_row(r, h);
-                if (d < p.head_dim) dqg[(int64_t)d * p.dqc] = (T)(valid ? acc[0][blk][r] * p.scale : 0.0f);
+                if (d < p.head_dim) dqg[(int64_t)d * p.dqc] = (T)(valid ? acc[blk][r] * p.scale : 0.0f);
             }
     }
     if (p.bias) {
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) { far_left += __shfl_xor(far_left, o); far_right += __shfl_xor(far_right, o); }
         wave_lds_fence();
-        if (l == 0) { hist[0] += far_left; hist[offsets - 1] += far_right; }
+        if (l == 0) { hist[0] = (float)((double)hist[0] + far_left); hist[offsets - 1] = (float)((double)hist[offsets - 1] + far_right); }
         __syncthreads();
         const float* all = tab + ((offsets + 3) & ~3);
         float* out = p.part_bias + ((int64_t)(head * p.batch + b) * p.tiles + qt) * offsets;
@@ -176,34 +218,48 @@ void bucket_dq_kernel(Dev p)
 
 // dk_j = scale * sum_i ds_ij q_i, dv_j = sum_i p_ij dout_i over all heads that share the kv head.  Scores
 // are untransposed here (rows = queries, columns = keys): a key is a lane.
-template <typename T, int DP>
-__global__ __launch_bounds__(NTHR)
+//
+// KW = 2: half of the waves take the first, half the second 32 queries of every tile (64 keys per workgroup).
+// The last workgroups of the launch do the sums of the bias gradient.
+__device__ void dbias_of_head(const Dev& p, int head, unsigned char* lds);
+
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(NTHR, (Shape<T, DP, KW>::MIN_WAVES))
 void bucket_dkv_kernel(Dev p)
 {
     using F = typename Num<T>::frag;
-    constexpr int KS = Num<T>::KS, PT = Num<T>::PT;
+    using S = Shape<T, DP, KW>;
+    constexpr int KT = S::KT, NS = S::NS, SP = S::SP, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, CW = NWAVE / KW;
     extern __shared__ __align__(16) unsigned char lds[];
+    if ((int)blockIdx.x >= p.kv_blocks) { dbias_of_head(p, (int)blockIdx.x - p.kv_blocks, lds); return; }
     T* qim = reinterpret_cast<T*>(lds);
     T* dim = qim + DP * PT;
     float* st = reinterpret_cast<float*>(dim + DP * PT);        // log-sum-exp and delta of the tile's queries
     float* tab = st + 2 * KT;
 
-    int unit, within;
-    if (!place(p, unit, within)) return;
-    const int kvh = unit % (p.heads / p.group), b = unit / (p.heads / p.group);
+    const Place at = place(p);
+    if (!at.any) return;
+    const int b = at.b, kvh = at.kvh;
     const Item it = item_of(p, b);
     const int l = threadIdx.x & 63, h = l >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int kt0 = within * NWAVE * 32, jb = kt0 + wave * 32, j = jb + (l & 31);
+    const int cw = wave / KW, kw = wave % KW;
+    const int kt0 = at.within * CW * 32, jb = kt0 + cw * 32, j = jb + (l & 31);
     const bool valid = j < it.nk;
 
-    F kf[1][DP / KS], vf[1][DP / KS];
-    load_frags<DP>(kf[0], (const T*)p.k + (int64_t)b * p.kb + (int64_t)kvh * p.head_dim * p.kc + j, p.kc, p.head_dim, valid);
-    load_frags<DP>(vf[0], (const T*)p.v + (int64_t)b * p.vb + (int64_t)kvh * p.head_dim * p.vc + j, p.vc, p.head_dim, valid);
-    f32x16 dk[1][DP / 32], dv[1][DP / 32];
+    F kf[DP / KS], vf[DP / KS];
+    if (kt0 < it.nk) {
+        OwnRows<T, DP, KT, CW> rk, rv;
+        const int64_t hd = (int64_t)kvh * p.head_dim;
+        rk.load((const T*)p.k + (int64_t)b * p.kb + hd * p.kc, p.kc, p.head_dim, kt0, it.nk);
+        rv.load((const T*)p.v + (int64_t)b * p.vb + hd * p.vc, p.vc, p.head_dim, kt0, it.nk);
+        rk.frags(kf, qim, dim, cw);
+        rv.frags(vf, qim, dim, cw);
+    }
+    f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { dk[0][blk][r] = 0.0f; dv[0][blk][r] = 0.0f; }
+        for (int r = 0; r < 16; ++r) { dk[blk][r] = 0.0f; dv[blk][r] = 0.0f; }
 
     // queries that see any of these keys: with `causal` those at or behind the first key
     int q_first = 0;
@@ -211,7 +267,7 @@ void bucket_dkv_kernel(Dev p)
     const int tiles = kt0 < it.nk ? (it.nq - q_first + KT - 1) / KT : 0;
     const int steps = tiles > 0 ? tiles * p.group : 0;
 
-    Tile<T, DP> qt, dt;
+    Tile<T, DP, KT> qt, dt;
     float stat = 0.0f;
     auto fetch = [&](int step) {
         const int g = step / tiles, i0 = q_first + (step - g * tiles) * KT;
@@ -239,40 +295,66 @@ void bucket_dkv_kernel(Dev p)
         __syncthreads();
         if (step + 1 < steps) fetch(step + 1);
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-            const int is = i0 + 32 * sub, pos0 = it.start + is;
-            if (is >= it.nq || (p.causal && jb > pos0 + 31)) continue;
-            f32x16 s[1], dp[1];
+        for (int sp = 0; sp < NS / SP; ++sp) {
+            const int c0 = 32 * (kw * NS + sp * SP), is = i0 + c0, pos0 = it.start + is;      // this step's queries
+            if (is >= it.nq || (p.causal && jb > pos0 + 32 * SP - 1)) continue;
+            const int lo = jb - (pos0 + 32 * SP - 1), hi = jb + 31 - pos0, side = bias_side(p, lo, hi);
+            f32x16 s[SP], dp[SP];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) { s[0][r] = 0.0f; dp[0][r] = -st[KT + 32 * sub + acc_row(r, h)]; }
-            dot_channels<DP, 1>(s, qim, 32 * sub, kf);
-            dot_channels<DP, 1>(dp, dim, 32 * sub, vf);
-            const int lo = jb - (pos0 + 31), hi = jb + 31 - pos0;
-            const BlockBias bb = block_bias(tab, p, lo, hi);
-            if (bb.near_) {
+            for (int i = 0; i < SP; ++i) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int off = clampi(j - (pos0 + acc_row(r, h)), -p.far_, p.far_);
-                    s[0][r] = fmaf(s[0][r], p.c, tab[off + p.far_] - st[32 * sub + acc_row(r, h)]);
-                }
+                for (int r = 0; r < 16; ++r) { s[i][r] = 0.0f; dp[i][r] = -st[KT + c0 + 32 * i + acc_row(r, h)]; }
+                dot_channels<DP, PT>(s[i], qim, c0 + 32 * i, kf);
+                dot_channels<DP, PT>(dp[i], dim, c0 + 32 * i, vf);
+            }
+            const float flat = bias_flat(tab, p, side);
+            if (side != BIAS_NEAR && !(p.causal && hi > 0)) {
+#pragma unroll
+                for (int i = 0; i < SP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        s[i][r] = exp2_hw(fmaf(s[i][r], p.c, flat - st[c0 + 32 * i + acc_row(r, h)]));
             } else {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], p.c, bb.flat - st[32 * sub + acc_row(r, h)]);
+                for (int i = 0; i < SP; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int row = 32 * i + acc_row(r, h), off = j - (pos0 + row);
+                        const float bias = side == BIAS_NEAR ? tab[clampi(off, -p.far_, p.far_) + p.far_] : flat;
+                        s[i][r] = exp2_hw(fmaf(s[i][r], p.c, bias - st[c0 + row]));
+                        if (p.causal && off > 0) s[i][r] = 0.0f;
+                    }
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[0][r] = exp2_hw(s[0][r]);
-            if (p.causal && hi > 0) {
+            for (int i = 0; i < SP; ++i) dot_positions<DP, PT>(dv, dim, c0 + 32 * i, s[i]);
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (j > pos0 + acc_row(r, h)) s[0][r] = 0.0f;
+            for (int i = 0; i < SP; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[i][r] *= dp[i][r];
+                dot_positions<DP, PT>(dk, qim, c0 + 32 * i, s[i]);
             }
-            dot_positions<DP, 1>(dv, dim, 32 * sub, s);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[0][r] *= dp[0][r];
-            dot_positions<DP, 1>(dk, qim, 32 * sub, s);
         }
     }
-    if (j < p.keys) {
+    if constexpr (KW == 2) {
+        float* red = reinterpret_cast<float*>(lds) + cw * DP * 32 + (l & 31);
+        auto join = [&](f32x16 (&x)[DP / 32]) {
+            __syncthreads();
+            if (kw == 1)
+#pragma unroll
+                for (int blk = 0; blk < DP / 32; ++blk)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) red[(32 * blk + acc_row(r, h)) * 32] = x[blk][r];
+            __syncthreads();
+            if (kw == 0)
+#pragma unroll
+                for (int blk = 0; blk < DP / 32; ++blk)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[blk][r] += red[(32 * blk + acc_row(r, h)) * 32];
+        };
+        join(dk);
+        join(dv);
+    }
+    if (j < p.keys && kw == 0) {
         const int64_t hd = (int64_t)kvh * p.head_dim;
         T* dkg = (T*)p.dk + (int64_t)b * p.dkb + hd * p.dkc + j;
         T* dvg = (T*)p.dv + (int64_t)b * p.dvb + hd * p.dvc + j;
@@ -282,71 +364,90 @@ void bucket_dkv_kernel(Dev p)
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * blk + acc_row(r, h);
                 if (d < p.head_dim) {
-                    dkg[(int64_t)d * p.dkc] = (T)(valid ? dk[0][blk][r] * p.scale : 0.0f);
-                    dvg[(int64_t)d * p.dvc] = (T)(valid ? dv[0][blk][r] : 0.0f);
+                    dkg[(int64_t)d * p.dkc] = (T)(valid ? dk[blk][r] * p.scale : 0.0f);
+                    dvg[(int64_t)d * p.dvc] = (T)(valid ? dv[blk][r] : 0.0f);
                 }
             }
     }
 }
 
-// dbias[h, c] = sum of the diagonal sums whose offset falls into bucket c, over all workgroups of head h.
-constexpr int BR_THREADS = 1024;
-__global__ __launch_bounds__(BR_THREADS)
-void bucket_dbias_kernel(const float* part, const int32_t* bucket_of, float* dbias, int parts, int far_, int buckets)
+// dbias[h, c] = sum of the diagonal sums whose offset falls into bucket c, over all workgroups of head h, in 64 bits
+// (the sums of a row cancel to zero).
+__device__ void dbias_of_head(const Dev& p, int head, unsigned char* lds)
 {
-    extern __shared__ float sums[];                     // [4][offsets]
-    const int offsets = 2 * far_ + 1, head = (int)blockIdx.x, tid = (int)threadIdx.x;
-    const float* src = part + (int64_t)head * parts * offsets;
-    const int lane = tid & 255, quarter = tid >> 8;
-    for (int o = lane; o < offsets; o += 256) {
-        float s = 0.0f;
-        for (int i = quarter; i < parts; i += 4) s += src[(int64_t)i * offsets + o];
-        sums[quarter * offsets + o] = s;
+    const int offsets = 2 * p.far_ + 1, tid = (int)threadIdx.x, parts = p.batch * p.tiles;
+    float* sums = reinterpret_cast<float*>(lds);
+    int* bucket = reinterpret_cast<int*>(sums + offsets);
+    const float* src = p.part_bias + (int64_t)head * parts * offsets;
+    for (int o = tid; o < offsets; o += NTHR) {
+        double s = 0.0;
+        int i = 0;
+        for (; i + 8 <= parts; i += 8) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = src[(int64_t)(i + e) * offsets + o];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += v[e];
+        }
+        for (; i < parts; ++i) s += src[(int64_t)i * offsets + o];
+        sums[o] = (float)s;
+        bucket[o] = clampi(p.bucket_of[o], 0, p.buckets - 1);
     }
     __syncthreads();
-    for (int c = tid; c < buckets; c += BR_THREADS) {
-        float s = 0.0f;
-        for (int o = 0; o < offsets; ++o) {
-            const int bk = clampi(bucket_of[o], 0, buckets - 1);
-            if (bk == c) s += (sums[o] + sums[offsets + o]) + (sums[2 * offsets + o] + sums[3 * offsets + o]);
-        }
-        dbias[(int64_t)head * buckets + c] = s;
+    for (int c0 = 0; c0 < p.buckets; c0 += NTHR / 32) {
+        const int c = c0 + tid / 32;
+        double s = 0.0;
+        for (int o = tid & 31; o < offsets; o += 32) s += bucket[o] == c ? (double)sums[o] : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor(s, o, 32);
+        if ((tid & 31) == 0 && c < p.buckets) p.dbias[(int64_t)head * p.buckets + c] = (float)s;
     }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int KW>
 int launch_both(Dev d, hipStream_t st)
 {
-    const size_t img = 2 * (size_t)Tile<T, DP>::BYTES, offsets = 2 * (size_t)d.far_ + 1;
+    const size_t img = 2 * (size_t)Tile<T, DP, Shape<T, DP, KW>::KT>::BYTES, offsets = 2 * (size_t)d.far_ + 1;
     const char* what = "vk_bucket_attention_backward";
+    constexpr int ROWS = NWAVE / KW * 32;
+    d.tiles = (d.queries + ROWS - 1) / ROWS;
     if (d.queries > 0) {
-        d.tiles = (d.queries + NWAVE * 32 - 1) / (NWAVE * 32);
         vkba_place(d, (int64_t)d.tiles * d.group);
         const size_t lds = img + vkba_table_bytes(d) + (d.bias ? NWAVE * (offsets + 32 * DGP) * 4 : 0);
-        int rc = vkba_launch<bucket_dq_kernel<T, DP>>(d, vkba_blocks(d), lds, st, what);
+        int rc = vkba_launch<bucket_dq_kernel<T, DP, KW>>(d, vkba_blocks(d), lds, st, what);
         if (rc != VK_OK) return rc;
     }
-    if (d.keys > 0) {
-        vkba_place(d, (d.keys + NWAVE * 32 - 1) / (NWAVE * 32));
-        return vkba_launch<bucket_dkv_kernel<T, DP>>(d, vkba_blocks(d), img + 2 * KT * 4 + vkba_table_bytes(d), st, what);
-    }
-    return VK_OK;
+    vkba_place(d, (d.keys + ROWS - 1) / ROWS);
+    const int64_t blocks = d.keys > 0 ? vkba_blocks(d) : 0;
+    if (blocks > 0x7fffffff) return vkba_fail(VK_E_UNSUPPORTED, what, "too many workgroups");
+    d.kv_blocks = (int)blocks;
+    const size_t need = img + 2 * Shape<T, DP, KW>::KT * 4 + vkba_table_bytes(d);
+    return vkba_launch<bucket_dkv_kernel<T, DP, KW>>(d, blocks + (d.bias ? d.heads : 0), need > offsets * 8 ? need : offsets * 8, st, what);
 }
 
-template <typename T>
+template <typename T, int KW>
 int by_width(const Dev& d, hipStream_t st)
 {
     switch ((d.head_dim + 31) / 32) {
-    case 1: return launch_both<T, 32>(d, st);
-    case 2: return launch_both<T, 64>(d, st);
-    case 3: return launch_both<T, 96>(d, st);
-    default: return launch_both<T, 128>(d, st);
+    case 1: return launch_both<T, 32, KW>(d, st);
+    case 2: return launch_both<T, 64, KW>(d, st);
+    case 3: return launch_both<T, 96, KW>(d, st);
+    default: return launch_both<T, 128, KW>(d, st);
     }
 }
 
+#ifndef KWB
+#define KWB 256
+#endif
+// Rows (queries of the first, keys of the second kernel) per workgroup.
+int key_waves(const vk_bucket_attention_args* a)
+{
+    return a->dtype == VK_DTYPE_F32 || (int64_t)a->batch * a->heads * ((a->queries + 127) / 128) < KWB ? 2 : 1;
+}
 int64_t parts_of_head(const vk_bucket_attention_args* a)
 {
-    return (int64_t)a->batch * ((a->queries + NWAVE * 32 - 1) / (NWAVE * 32));
+    const int rows = 128 / key_waves(a);
+    return (int64_t)a->batch * ((a->queries + rows - 1) / rows);
 }
 int64_t workspace_floats(const vk_bucket_attention_args* a)
 {
@@ -382,15 +483,8 @@ extern "C" int vk_bucket_attention_backward(const vk_bucket_attention_args* a, v
         return vkba_fail(VK_E_WORKSPACE, what, "workspace smaller than vk_bucket_attention_backward_workspace_bytes");
     d.delta = (float*)a->workspace;
     d.part_bias = d.delta + (int64_t)a->batch * a->heads * a->queries;
+    d.dbias = a->dbias;
     hipStream_t st = (hipStream_t)stream;
-    if (a->batch > 0) {
-        rc = a->dtype == VK_DTYPE_BF16 ? by_width<__bf16>(d, st) : by_width<float>(d, st);
-        if (rc != VK_OK) return rc;
-    }
-    if (!a->has_bias) return VK_OK;
-    const size_t lds = 4 * (2 * (size_t)a->max_distance + 1) * 4;
-    hipLaunchKernelGGL(bucket_dbias_kernel, dim3((unsigned)a->heads), dim3(BR_THREADS), lds, st, d.part_bias, a->bucket_of,
-                       a->dbias, (int)parts_of_head(a), a->max_distance, a->buckets);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? VK_OK : vkba_fail(VK_E_LAUNCH, what, hipGetErrorString(e));
+    if (key_waves(a) == 2) return a->dtype == VK_DTYPE_BF16 ? by_width<__bf16, 2>(d, st) : by_width<float, 2>(d, st);
+    return by_width<__bf16, 1>(d, st);
 }

@@ -1,6 +1,6 @@
 // Forward pass of the bucketed-bias attention.  See bucket_attention.hpp for the data layout.
 //
-// A workgroup owns 4 * 32 * NQ queries of one head and walks over the keys in tiles of 64, one pass,
+// A workgroup owns 128 or 64 queries of one head and walks over the keys in tiles of 64, one pass,
 // with the running maximum and sum of the softmax.  Scores are computed transposed (rows = keys,
 // columns = queries), so a query is a lane: its maximum and sum are lane-local but for one exchange
 // between the two lane halves, and the probabilities are already the right operand of P V.
@@ -11,30 +11,41 @@
 namespace {
 using namespace vkba;
 
-template <typename T, int DP, int NQ>
-__global__ __launch_bounds__(NTHR)
+constexpr int FWD_TILE = 64;    // keys of a staged tile
+
+// KW = 2: half of the waves take the first, half the second 32 keys of every tile (64 queries per workgroup
+// instead of 128), each with a maximum, sum and output of its own, joined through LDS at the end.  The staging of
+// a tile is then shared by half the work, but there are twice the workgroups.
+template <typename T, int DP, int KW>
+#ifndef BW64
+#define BW64 3
+#endif
+#ifndef FW
+#define FW 2
+#endif
+__global__ __launch_bounds__(NTHR, sizeof(T) == 4 ? FW : (DP <= 64 ? BW64 : 2))
 void bucket_attention_kernel(Dev p)
 {
     using F = typename Num<T>::frag;
-    constexpr int KS = Num<T>::KS, PT = Num<T>::PT, QT = NWAVE * 32 * NQ;
+    constexpr int KT = FWD_TILE, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, QW = NWAVE / KW, QT = QW * 32;
+    constexpr int NS = KT / 32 / KW;                              // 32-key blocks of a tile per wave
+    constexpr int SP = sizeof(T) == 4 ? 1 : NS;             // of them in one softmax step (fp32: 1, to keep the registers)
     extern __shared__ __align__(16) unsigned char lds[];
     T* ki = reinterpret_cast<T*>(lds);
     T* vi = ki + DP * PT;
     float* tab = reinterpret_cast<float*>(vi + DP * PT);
 
-    int unit, within;
-    if (!place(p, unit, within)) return;
-    const int kvh = unit % (p.heads / p.group), b = unit / (p.heads / p.group);
-    const int g = within % p.group;
-    int rest = within / p.group;
+    const Place at = place(p);
+    if (!at.any) return;
+    const int b = at.b, kvh = at.kvh, g = at.within % p.group, rest = at.within / p.group;
     const int split = rest % p.splits;
-    const int qt = p.tiles - 1 - rest / p.splits;          // causal: the longest rows first
+    const int qt = p.tiles - 1 - rest / p.splits;           // causal: the longest rows first
     const int head = kvh * p.group + g;
     const Item it = item_of(p, b);
     const int l = threadIdx.x & 63, h = l >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int q0 = qt * QT + wave * 32 * NQ;
+    const int qw = wave / KW, kw = wave % KW;
+    const int q0 = qt * QT + qw * 32, qi = q0 + (l & 31);
 
-    const T* qg = (const T*)p.q + (int64_t)b * p.qb + (int64_t)head * p.head_dim * p.qc;
     const T* kg = (const T*)p.k + (int64_t)b * p.kb + (int64_t)kvh * p.head_dim * p.kc;
     const T* vg = (const T*)p.v + (int64_t)b * p.vb + (int64_t)kvh * p.head_dim * p.vc;
 
@@ -46,32 +57,26 @@ void bucket_attention_kernel(Dev p)
     const int first = split * p.per_split * KT;
     end = min(end, first + p.per_split * KT);
 
-    F qf[NQ][DP / KS];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int qi = q0 + 32 * n + (l & 31);
-        load_frags<DP>(qf[n], qg + qi, p.qc, p.head_dim, qi < it.nq);
-    }
-    stage_bias(tab, p, head);
-
-    f32x16 acc[NQ][DP / 32];
-    float m[NQ], sum[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        m[n] = -__builtin_inff();
-        sum[n] = 0.0f;
-#pragma unroll
-        for (int blk = 0; blk < DP / 32; ++blk)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[n][blk][r] = 0.0f;
-    }
-
-    Tile<T, DP> kt, vt;
+    Tile<T, DP, KT> kt, vt;
+    F qf[DP / KS];
     if (first < end) {
+        OwnRows<T, DP, KT, QW> rows;
+        rows.load((const T*)p.q + (int64_t)b * p.qb + (int64_t)head * p.head_dim * p.qc, p.qc, p.head_dim, qt * QT, it.nq);
         kt.load(kg, p.kc, p.head_dim, first, end);
         vt.load(vg, p.vc, p.head_dim, first, end);
+        stage_bias(tab, p, head);
+        rows.frags(qf, ki, vi, qw);
     }
+
+    f32x16 acc[DP / 32];
+    float m = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+    for (int blk = 0; blk < DP / 32; ++blk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[blk][r] = 0.0f;
+
     const float c = p.c;
+    const int pos0 = it.start + q0, pos = pos0 + (l & 31);
     for (int j0 = first; j0 < end; j0 += KT) {
         __syncthreads();
         kt.store(ki);
@@ -81,103 +86,125 @@ void bucket_attention_kernel(Dev p)
             kt.load(kg, p.kc, p.head_dim, j0 + KT, end);
             vt.load(vg, p.vc, p.head_dim, j0 + KT, end);
         }
-        const int pos0 = it.start + q0;
-        if (p.causal && j0 > pos0 + 32 * NQ - 1) continue;      // this wave's queries see none of the tile
-        f32x16 s[2][NQ];
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
+        for (int step = 0; step < NS / SP; ++step) {
+            const int c0 = 32 * (kw * NS + step * SP), js = j0 + c0;            // this step's keys: SP * 32 from here
+            if (js >= end || (p.causal && js > pos0 + 31)) continue;            // none in sight of this wave
+            f32x16 s[SP];
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
+            for (int i = 0; i < SP; ++i) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[sub][n][r] = 0.0f;
-            dot_channels<DP, NQ>(s[sub], ki, 32 * sub, qf);
-        }
+                for (int r = 0; r < 16; ++r) s[i][r] = 0.0f;
+                dot_channels<DP, PT>(s[i], ki, c0 + 32 * i, qf);
+            }
+            float mul = c, flat = 0.0f;                                         // logit = mul * s + flat
+            const int lo = js - (pos0 + 31), hi = js + 32 * SP - 1 - pos0;
+            const int side = bias_side(p, lo, hi);
+            if (side == BIAS_NEAR) {
+                mul = 1.0f;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const int pos = pos0 + 32 * n + (l & 31);
-            float mx = m[n];
-#pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                const int js = j0 + 32 * sub;
-                const int lo = js - (pos0 + 32 * n + 31), hi = js + 31 - (pos0 + 32 * n);
-                const BlockBias bb = block_bias(tab, p, lo, hi);
-                if (bb.near_) {
+                for (int i = 0; i < SP; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int off = clampi(js + acc_row(r, h) - pos, -p.far_, p.far_);
-                        s[sub][n][r] = fmaf(s[sub][n][r], c, tab[off + p.far_]);
+                        const int off = clampi(js + 32 * i + acc_row(r, h) - pos, -p.far_, p.far_);
+                        s[i][r] = fmaf(s[i][r], c, tab[off + p.far_]);
                     }
-                } else {
+            } else {
+                flat = bias_flat(tab, p, side);
+            }
+            if (js + 32 * SP > end || (p.causal && hi > 0)) {
+                const int stop = (p.causal ? min(end, pos + 1) : end) - js;
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s[sub][n][r] = fmaf(s[sub][n][r], c, bb.flat);
-                }
-                if (js + 32 > end || (p.causal && hi > 0)) {
-                    const int stop = p.causal ? min(end, pos + 1) : end;
+                for (int i = 0; i < SP; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (js + acc_row(r, h) >= stop) s[sub][n][r] = -__builtin_inff();
-                }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[sub][n][r]);
+                        if (32 * i + acc_row(r, h) >= stop) s[i][r] = -__builtin_inff();
             }
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 0; i < SP; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float base = mx == -__builtin_inff() ? 0.0f : mx;
-            if (__any(mx > m[n])) {                             // the maximum moved for some query of the wave
-                const float alpha = exp2_hw(m[n] - base);
-                sum[n] *= alpha;
+            mx = fmaf(mx, mul, flat);                                           // the scale is positive: the maximum stays the maximum
+            // m is the exponents' reference, not the exact maximum: it follows when some query of the wave is more
+            // than 8 (a factor of 256) above it, so that the sums and the output are rarely scaled anew
+            if (__any(mx > m + 8.0f)) {
+                const float top = fmaxf(mx, m), alpha = exp2_hw(m - (top == -__builtin_inff() ? 0.0f : top));
+                sum *= alpha;
 #pragma unroll
                 for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[n][blk][r] *= alpha;
-                m[n] = mx;
+                    for (int r = 0; r < 16; ++r) acc[blk][r] *= alpha;
+                m = top;
             }
+            const float base = m == -__builtin_inff() ? 0.0f : m;
+            const float shift = flat - base;
             float add = 0.0f;
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub)
+            for (int i = 0; i < SP; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[sub][n][r] = exp2_hw(s[sub][n][r] - base);
-                    add += s[sub][n][r];
+                    s[i][r] = exp2_hw(fmaf(s[i][r], mul, shift));
+                    add += s[i][r];
                 }
-            sum[n] += add;
-        }
+            sum += add;
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) dot_positions<DP, NQ>(acc, vi, 32 * sub, s[sub]);
+            for (int i = 0; i < SP; ++i) dot_positions<DP, PT>(acc, vi, c0 + 32 * i, s[i]);
+        }
     }
 
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const int qi = q0 + 32 * n + (l & 31);
-        const float total = sum[n] + __shfl_xor(sum[n], 32);
-        if (qi >= p.queries) continue;
-        const bool live = qi < it.nq && total > 0.0f;
-        const bool broken = qi < it.nq && !(total >= 0.0f);     // NaN in the inputs stays visible
-        const int64_t row = ((int64_t)b * p.heads + head) * p.queries + qi;
-        if (p.splits == 1) {
-            const float inv = live || broken ? 1.0f / total : 0.0f;
-            T* og = (T*)p.out + (int64_t)b * p.ob + (int64_t)head * p.head_dim * p.oc + qi;
+    float total = sum + __shfl_xor(sum, 32);
+    if constexpr (KW == 2) {
+        __syncthreads();                                    // the images are free
+        float* red = reinterpret_cast<float*>(lds) + qw * (DP + 2) * 32 + (l & 31);
+        if (kw == 1) {
 #pragma unroll
             for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = 32 * blk + acc_row(r, h);
-                    if (d < p.head_dim) og[(int64_t)d * p.oc] = (T)(live || broken ? acc[n][blk][r] * inv : 0.0f);
-                }
-            if (h == 0) p.lse[row] = live || broken ? (m[n] + log2f(total)) * LN2 : -__builtin_inff();
-        } else {
-            const int64_t rows = (int64_t)p.batch * p.heads * p.queries;
-            float* po = p.part_o + ((int64_t)split * p.batch * p.heads + (int64_t)b * p.heads + head) * p.head_dim * p.queries + qi;
+                for (int r = 0; r < 16; ++r) red[(32 * blk + acc_row(r, h)) * 32] = acc[blk][r];
+            red[DP * 32] = m;
+            red[(DP + 1) * 32] = total;
+        }
+        __syncthreads();
+        if (kw == 1) return;
+        const float m1 = red[DP * 32], t1 = red[(DP + 1) * 32];
+        const float mx = fmaxf(m, m1), base = mx == -__builtin_inff() ? 0.0f : mx;
+        const float w0 = exp2_hw(m - base), w1 = exp2_hw(m1 - base);
+        m = mx;
+        total = total * w0 + t1 * w1;
 #pragma unroll
-            for (int blk = 0; blk < DP / 32; ++blk)
+        for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = 32 * blk + acc_row(r, h);
-                    if (d < p.head_dim) po[(int64_t)d * p.queries] = acc[n][blk][r];
-                }
-            if (h == 0) {
-                p.part_ml[((int64_t)split * rows + row) * 2] = qi < it.nq ? m[n] : -__builtin_inff();
-                p.part_ml[((int64_t)split * rows + row) * 2 + 1] = qi < it.nq ? total : 0.0f;
+            for (int r = 0; r < 16; ++r) acc[blk][r] = acc[blk][r] * w0 + red[(32 * blk + acc_row(r, h)) * 32] * w1;
+    }
+    if (qi >= p.queries) return;
+    const bool some = qi < it.nq && !(total == 0.0f);       // NaN in the inputs stays visible
+    const int64_t row = ((int64_t)b * p.heads + head) * p.queries + qi;
+    if (p.splits == 1) {
+        const float inv = 1.0f / total;
+        T* og = (T*)p.out + (int64_t)b * p.ob + (int64_t)head * p.head_dim * p.oc + qi;
+#pragma unroll
+        for (int blk = 0; blk < DP / 32; ++blk)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * blk + acc_row(r, h);
+                if (d < p.head_dim) og[(int64_t)d * p.oc] = (T)(some ? acc[blk][r] * inv : 0.0f);
             }
+        if (h == 0) p.lse[row] = some ? (m + log2f(total)) * LN2 : -__builtin_inff();
+    } else {
+        const int64_t rows = (int64_t)p.batch * p.heads * p.queries;
+        float* po = p.part_o + ((int64_t)split * p.batch * p.heads + (int64_t)b * p.heads + head) * p.head_dim * p.queries + qi;
+#pragma unroll
+        for (int blk = 0; blk < DP / 32; ++blk)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int d = 32 * blk + acc_row(r, h);
+                if (d < p.head_dim) po[(int64_t)d * p.queries] = acc[blk][r];
+            }
+        if (h == 0) {
+            p.part_ml[((int64_t)split * rows + row) * 2] = some ? m : -__builtin_inff();
+            p.part_ml[((int64_t)split * rows + row) * 2 + 1] = some ? total : 0.0f;
         }
     }
 }
@@ -214,36 +241,41 @@ void bucket_attention_join_kernel(Dev p)
     if (d == 0) p.lse[row] = none ? -__builtin_inff() : (m + log2f(total)) * LN2;
 }
 
-template <typename T, int DP, int NQ>
-int launch(const Dev& d, hipStream_t st)
+template <typename T, int DP>
+int launch(const Dev& d, int kw, hipStream_t st)
 {
-    const size_t lds = 2 * (size_t)Tile<T, DP>::BYTES + vkba_table_bytes(d);
-    return vkba_launch<bucket_attention_kernel<T, DP, NQ>>(d, vkba_blocks(d), lds, st, "vk_bucket_attention");
+    const size_t lds = 2 * (size_t)Tile<T, DP, FWD_TILE>::BYTES + vkba_table_bytes(d);
+    if constexpr (sizeof(T) == 2)
+        if (kw == 1) return vkba_launch<bucket_attention_kernel<T, DP, 1>>(d, vkba_blocks(d), lds, st, "vk_bucket_attention");
+    return vkba_launch<bucket_attention_kernel<T, DP, 2>>(d, vkba_blocks(d), lds, st, "vk_bucket_attention");
 }
 
-template <typename T, int NQ>
-int by_width(const Dev& d, hipStream_t st)
+template <typename T>
+int by_width(const Dev& d, int kw, hipStream_t st)
 {
     switch ((d.head_dim + 31) / 32) {
-    case 1: return launch<T, 32, NQ>(d, st);
-    case 2: return launch<T, 64, NQ>(d, st);
-    case 3: return launch<T, 96, NQ>(d, st);
-    default: return launch<T, 128, NQ>(d, st);
+    case 1: return launch<T, 32>(d, kw, st);
+    case 2: return launch<T, 64>(d, kw, st);
+    case 3: return launch<T, 96>(d, kw, st);
+    default: return launch<T, 128>(d, kw, st);
     }
 }
 
-}  // namespace
-
-// Queries per workgroup and shares of the keys' length.  512 workgroups keep two on every CU; with
-// fewer the key axis is cut, down to two tiles per share.
-static void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& nq)
+// Queries per workgroup (128 or, with the waves in two key halves, 64) and shares of the keys' length.
+#ifndef KWB
+#define KWB 256
+#endif
+#ifndef SPB
+#define SPB 256
+#endif
+void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& kw)
 {
     const int64_t heads = (int64_t)a->batch * a->heads;
-    nq = a->dtype == VK_DTYPE_BF16 && heads * ((a->queries + 255) / 256) >= 512 ? 2 : 1;
-    d.tiles = (a->queries + 128 * nq - 1) / (128 * nq);
+    kw = a->dtype == VK_DTYPE_F32 || heads * ((a->queries + 127) / 128) < KWB ? 2 : 1;
+    d.tiles = (a->queries + 128 / kw - 1) / (128 / kw);
     const int64_t blocks = heads * d.tiles;
-    const int key_tiles = (a->keys + KT - 1) / KT;
-    int64_t splits = blocks >= 256 || blocks == 0 ? 1 : (512 + blocks - 1) / blocks;
+    const int key_tiles = (a->keys + FWD_TILE - 1) / FWD_TILE;
+    int64_t splits = blocks >= SPB || blocks == 0 ? 1 : (2 * SPB + blocks - 1) / blocks;
     splits = splits > (key_tiles + 1) / 2 ? (key_tiles + 1) / 2 : splits;
     if (splits < 1) splits = 1;
     d.per_split = (int)((key_tiles + splits - 1) / splits);
@@ -253,33 +285,34 @@ static void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& nq)
     vkba_place(d, (int64_t)d.tiles * d.splits * d.group);
 }
 
+}  // namespace
+
 extern "C" int64_t vk_bucket_attention_workspace_bytes(const vk_bucket_attention_args* a)
 {
     vkba::Dev d;
-    int rc = vkba_check(a, d, "vk_bucket_attention_workspace_bytes", false), nq;
+    int rc = vkba_check(a, d, "vk_bucket_attention_workspace_bytes", false), kw;
     if (rc != VK_OK) return rc;
-    plan_forward(a, d, nq);
+    plan_forward(a, d, kw);
     return d.splits > 1 ? (int64_t)d.splits * a->batch * a->heads * a->queries * (a->head_dim + 2) * 4 : 0;
 }
 
 extern "C" int vk_bucket_attention(const vk_bucket_attention_args* a, void* stream)
 {
-    Dev d;
-    int rc = vkba_check(a, d, "vk_bucket_attention", true), nq;
+    vkba::Dev d;
+    int rc = vkba_check(a, d, "vk_bucket_attention", true), kw;
     if (rc != VK_OK) return rc;
     if (a->batch == 0 || a->queries == 0) return VK_OK;
     if (!a->out || !a->lse) return vk_fail(VK_E_ARG, "vk_bucket_attention: null output");
     if (!vkba_rows_apart(a->out_bstride, a->out_cstride, (int64_t)a->heads * a->head_dim, a->queries, a->batch))
         return vk_fail(VK_E_ARG, "vk_bucket_attention: rows of out overlap");
-    plan_forward(a, d, nq);
+    plan_forward(a, d, kw);
     const int64_t need = d.splits > 1 ? (int64_t)d.splits * a->batch * a->heads * a->queries * (a->head_dim + 2) * 4 : 0;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need))
         return vk_fail(VK_E_WORKSPACE, "vk_bucket_attention: workspace smaller than vk_bucket_attention_workspace_bytes");
     d.part_ml = (float*)a->workspace;
     d.part_o = d.part_ml + (int64_t)d.splits * a->batch * a->heads * a->queries * 2;
     hipStream_t st = (hipStream_t)stream;
-    rc = a->dtype == VK_DTYPE_BF16 ? (nq == 2 ? by_width<__bf16, 2>(d, st) : by_width<__bf16, 1>(d, st))
-                                   : by_width<float, 1>(d, st);
+    rc = a->dtype == VK_DTYPE_BF16 ? by_width<__bf16>(d, kw, st) : by_width<float>(d, kw, st);
     if (rc != VK_OK || d.splits == 1) return rc;
     const int64_t n = (int64_t)a->batch * a->heads * a->head_dim * a->queries;
     dim3 grid((unsigned)((n + 255) / 256));

@@ -32,7 +32,7 @@ inline int vkba_check(const vk_bucket_attention_args* a, vkba::Dev& d, const cha
     if (a->dtype != VK_DTYPE_F32 && a->dtype != VK_DTYPE_BF16) return vkba_fail(VK_E_UNSUPPORTED, what, "dtype must be VK_DTYPE_F32 or VK_DTYPE_BF16");
     if (a->head_dim < 1 || a->head_dim > VK_BUCKET_MAX_HEAD_DIM) return vkba_fail(VK_E_UNSUPPORTED, what, "head_dim must be 1..128");
     if (a->queries > VK_BUCKET_MAX_LENGTH || a->keys > VK_BUCKET_MAX_LENGTH) return vkba_fail(VK_E_UNSUPPORTED, what, "length beyond VK_BUCKET_MAX_LENGTH");
-    if (!(fabsf(a->scale) < 1e30f)) return vkba_fail(VK_E_ARG, what, "scale must be finite");
+    if (!(a->scale > 0.0f && a->scale < 1e30f)) return vkba_fail(VK_E_ARG, what, "scale must be positive and finite");
     if (a->has_bias && (a->buckets < 1 || a->max_distance < 1 || a->max_distance > VK_BUCKET_MAX_DISTANCE))
         return vkba_fail(VK_E_UNSUPPORTED, what, "bias needs at least one bucket and max_distance in 1..VK_BUCKET_MAX_DISTANCE");
     if (pointers) {
@@ -71,6 +71,7 @@ inline void vkba_place(vkba::Dev& d, int64_t per_unit)
     d.per_unit = (int)(per_unit > 0x7fffffff ? 0x7fffffff : per_unit);
     const int64_t rounds = (d.units + 7) / 8;
     d.spread = d.units >= 8 && rounds * 8 * 10 <= (int64_t)d.units * 11;
+    d.sort = (d.nk || d.nq) && d.batch > 1 && d.batch <= 64;
 }
 inline int64_t vkba_blocks(const vkba::Dev& d)
 {
