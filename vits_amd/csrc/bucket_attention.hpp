@@ -251,6 +251,21 @@ __device__ __forceinline__ void dot_positions(f32x16 (&acc)[DP / 32], const floa
         }
 }
 
+template <int N>
+__device__ __forceinline__ void flip(bf16x8 (&f)[N], bool neg)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[i][e] = neg ? -f[i][e] : f[i][e];
+}
+template <int N>
+__device__ __forceinline__ void flip(float (&f)[N], bool neg)
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = neg ? -f[i] : f[i];
+}
+
 // Row (position within 32) of accumulator register r in lane half h.
 __device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
@@ -267,7 +282,7 @@ struct Dev {
     int units, spread, sort;        // (item, kv head) pairs; 1: a pair's workgroups on one XCD; 1: items by their work
     int per_unit;
     float* part_o; float* part_ml;  // forward: partial results of the shares
-    float* dbias; int kv_blocks;    // backward: bias gradient, workgroups before those that sum it
+    float* dbias; int kv_blocks, fold;   // backward: bias gradient; workgroups before those that sum it; the order of the dv ones
     float* delta; float* part_bias; // backward: row sums of out * dout; diagonal sums of the logit gradients
 };
 
@@ -284,14 +299,24 @@ __device__ __forceinline__ Item item_of(const Dev& p, int b)
     return it;
 }
 
+// The same for the workgroup's own item, in scalar registers: everything that branches on it is uniform.
+__device__ __forceinline__ Item uniform_item(const Dev& p, int b)
+{
+    Item it = item_of(p, b);
+    it.nk = __builtin_amdgcn_readfirstlane(it.nk);
+    it.nq = __builtin_amdgcn_readfirstlane(it.nq);
+    it.start = __builtin_amdgcn_readfirstlane(it.start);
+    return it;
+}
+
 // Workgroup -> (item, kv head, index within the pair).  Workgroups go round robin over the 8 XCDs; with `spread` all
 // workgroups of a pair share one XCD, so the keys and values of a head stay in that XCD's L2 (pairs are dealt back and
 // forth, 0..7 then 7..0).  With lengths, items go in the order of their work, the largest first: the XCDs then get
 // like shares, and what starts last is short.
 struct Place { int b, kvh, within; bool any; };
-__device__ __forceinline__ Place place(const Dev& p)
+__device__ __forceinline__ Place place(const Dev& p, int id)
 {
-    const int id = (int)blockIdx.x, kv_heads = p.heads / p.group;
+    const int kv_heads = p.heads / p.group;
     int unit;
     Place r;
     if (p.spread) {
@@ -302,6 +327,8 @@ __device__ __forceinline__ Place place(const Dev& p)
         unit = id / p.per_unit;
         r.within = id - unit * p.per_unit;
     }
+    unit = __builtin_amdgcn_readfirstlane(unit);
+    r.within = __builtin_amdgcn_readfirstlane(r.within);
     r.any = unit < p.units;
     r.b = unit / kv_heads;
     r.kvh = unit - r.b * kv_heads;
@@ -315,7 +342,7 @@ __device__ __forceinline__ Place place(const Dev& p)
             rank += other > mine || (other == mine && o < lane);
         }
         const unsigned long long hit = __ballot(lane < p.batch && rank == r.b);
-        r.b = hit ? (int)__builtin_ctzll(hit) : 0;          // ranks are a permutation: there is exactly one
+        r.b = __builtin_amdgcn_readfirstlane(hit ? (int)__builtin_ctzll(hit) : 0);     // ranks are a permutation: exactly one
     }
     return r;
 }

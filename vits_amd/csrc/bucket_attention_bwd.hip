@@ -10,18 +10,20 @@
 namespace {
 using namespace vkba;
 
-// Waves per SIMD a kernel is built for, positions of a staged tile, 32-position blocks taken in one step.  Up to 96
-// channels (fp32: 64) two waves fit a SIMD's registers and one computes while the other waits; wider heads run one
-// wave with two blocks in one step instead.
+// How a kernel is built: waves per SIMD, positions of a staged tile, whether dk and dv have workgroups of their own.
+// Two waves per SIMD (at most 256 registers each) matter most: one computes while the other waits.  With bf16 and 128
+// channels dq fits with tiles of 32 keys (4096 positions, 16 heads: 806 -> 522 us), while dk and dv together with the
+// fragments of k and v do not fit at all and are computed by separate workgroups, for one more product (S twice).
 template <typename T, int DP, int KW>
 struct Shape {
-    static constexpr bool WIDE = sizeof(T) == 2 ? DP > 96 : DP > 64;
-    static constexpr int MIN_WAVES = WIDE ? 1 : 2;
-#ifndef WKT
-#define WKT 64
-#endif
-    static constexpr int KT = WIDE && sizeof(T) == 2 && KW == 2 ? WKT : 64;
-    static constexpr int NS = KT / 32 / KW, SP = WIDE ? NS : 1;
+    static constexpr bool BF = sizeof(T) == 2;
+    static constexpr bool SPLIT = BF && DP > 96;
+    static constexpr int MIN_WAVES = BF || DP <= 64 ? 2 : 1;
+    // the next tile is loaded into registers while the present one is computed, unless they make the second wave
+    static constexpr bool AHEAD = BF || MIN_WAVES == 1;
+    static constexpr int KT_DQ = BF && DP > 96 && KW == 1 ? 32 : 64, KT_DKV = KT_DQ;
+    static constexpr int OWN = Tile<T, DP, 64>::BYTES;                  // image of 64 of the workgroup's own rows
+    static constexpr int IMAGES = 2 * OWN;                              // as large as two tiles
 };
 
 constexpr int DGP = 33;         // pitch of a wave's 32 x 32 block of logit gradients
@@ -37,21 +39,22 @@ void bucket_dq_kernel(Dev p)
 {
     using F = typename Num<T>::frag;
     using S = Shape<T, DP, KW>;
-    constexpr int KT = S::KT, NS = S::NS, SP = S::SP, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, QW = NWAVE / KW, QT = QW * 32;
+    constexpr int KT = S::KT_DQ, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, QW = NWAVE / KW, QT = QW * 32;
     extern __shared__ __align__(16) unsigned char lds[];
     T* ki = reinterpret_cast<T*>(lds);
-    T* vi = ki + DP * PT;
-    float* tab = reinterpret_cast<float*>(vi + DP * PT);
+    T* vi = reinterpret_cast<T*>(lds + Tile<T, DP, KT>::BYTES);
+    T* own = reinterpret_cast<T*>(lds + S::OWN);            // second image of own rows
+    float* tab = reinterpret_cast<float*>(lds + S::IMAGES);
     const int offsets = 2 * p.far_ + 1;
     const int l = threadIdx.x & 63, h = l >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     float* hist = tab + ((offsets + 3) & ~3) + wave * offsets;                  // this wave's diagonal sums
     float* blk_ds = tab + ((offsets + 3) & ~3) + NWAVE * offsets + wave * 32 * DGP;
 
-    const Place at = place(p);
+    const Place at = place(p, (int)blockIdx.x);
     if (!at.any) return;
     const int b = at.b, kvh = at.kvh, head = kvh * p.group + at.within % p.group;
     const int qt = p.tiles - 1 - at.within / p.group;
-    const Item it = item_of(p, b);
+    const Item it = uniform_item(p, b);
     const int qw = wave / KW, kw = wave % KW;
     const int q0 = qt * QT + qw * 32, qi = q0 + (l & 31);
     const bool valid = qi < it.nq;
@@ -71,26 +74,39 @@ void bucket_dq_kernel(Dev p)
     // delta enters every logit gradient of its row with the same sign, so its error adds up coherently in the
     // bias gradient: summed in 64 bits, rounded once
     float delta = 0.0f;
+    // The matrix instruction's rounding leans to one side by some 1e-9 of a product sum, which shows in a bias gradient
+    // summed over 10^7 pairs (far bucket of 4095 causal positions: off by 6e-6 of its value).  Every other query takes
+    // its gradient with the other sign, so that the lean cancels; the results are turned back at the end.
+    const float sgn = (l & 1) ? -1.0f : 1.0f;
     if (qt * QT < it.nq) {
-        OwnRows<T, DP, KT, QW> rq, rd;
+        OwnRows<T, DP, 64, QW> rq, rd;
         rq.load((const T*)p.o + (int64_t)b * p.ob + hd * p.oc, p.oc, p.head_dim, qt * QT, it.nq);
         rd.load((const T*)p.dout + (int64_t)b * p.dob + hd * p.doc, p.doc, p.head_dim, qt * QT, it.nq);
-        rq.frags(qf, ki, vi, qw);
+        rq.frags(qf, ki, own, qw);
         rq.load((const T*)p.q + (int64_t)b * p.qb + hd * p.qc, p.qc, p.head_dim, qt * QT, it.nq);
-        rd.frags(dof, ki, vi, qw);
+        rd.frags(dof, ki, own, qw);
         delta = (float)dot_frags(qf, dof);
-        if (end > 0) {
+        flip(dof, sgn < 0.0f);
+        if (S::AHEAD && end > 0) {
             kt.load(kg, p.kc, p.head_dim, 0, end);
             vt.load(vg, p.vc, p.head_dim, 0, end);
         }
-        rq.frags(qf, ki, vi, qw);
+        rq.frags(qf, ki, own, qw);
     }
+    // lse2 rounds the row's log-sum-exp in units of log2: a relative error of some 1e-6 that all probabilities of the
+    // row share, so it does not average out in the bias gradient.  `off` is that error (below; 64 bits).
     float lse2 = __builtin_inff();
+    double off = 0.0;
     if (valid) {
         const float v = p.lse_in[row];
-        lse2 = v == -__builtin_inff() ? __builtin_inff() : v * LOG2E;          // no keys: all probabilities 0
+        if (v != -__builtin_inff()) {                       // without keys all probabilities are 0
+            lse2 = v * LOG2E;
+            off = (double)v * 1.4426950408889634 - (double)lse2;
+        }
         if (h == 0 && kw == 0) p.delta[row] = delta;
     }
+    const float near_fix = sgn * (float)(1.0 - off * (double)LN2);
+    const float minus_delta = -sgn * delta;
     stage_bias(tab, p, head);
     if (p.bias) for (int o = l; o < offsets; o += 64) hist[o] = 0.0f;
 
@@ -99,82 +115,74 @@ void bucket_dq_kernel(Dev p)
     for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[blk][r] = 0.0f;
-    double far_left = 0.0, far_right = 0.0;
+    double far_left = 0.0, far_right = 0.0;                // this query's sums over the whole blocks beyond the table
+    float end_left = 0.0f, end_right = 0.0f;                // of diagonals beyond it in blocks that reach into it
 
     const int pos0 = it.start + q0, pos = pos0 + (l & 31);
     for (int j0 = 0; j0 < end; j0 += KT) {
+        if constexpr (!S::AHEAD) {
+            kt.load(kg, p.kc, p.head_dim, j0, end);
+            vt.load(vg, p.vc, p.head_dim, j0, end);
+        }
         __syncthreads();
         kt.store(ki);
         vt.store(vi);
         __syncthreads();
-        if (j0 + KT < end) {
+        if (S::AHEAD && j0 + KT < end) {
             kt.load(kg, p.kc, p.head_dim, j0 + KT, end);
             vt.load(vg, p.vc, p.head_dim, j0 + KT, end);
         }
 #pragma unroll
-        for (int step = 0; step < NS / SP; ++step) {
-            const int c0 = 32 * (kw * NS + step * SP), js = j0 + c0;            // this step's keys: SP * 32 from here
+        for (int i = 0; i < KT / 32 / KW; ++i) {
+            const int c0 = 32 * (kw * (KT / 32 / KW) + i), js = j0 + c0;
             if (js >= end || (p.causal && js > pos0 + 31)) continue;
-            const int lo = js - (pos0 + 31), hi = js + 32 * SP - 1 - pos0, side = bias_side(p, lo, hi);
-            f32x16 s[SP], dp[SP];
+            const int lo = js - (pos0 + 31), hi = js + 31 - pos0, side = bias_side(p, lo, hi);
+            f32x16 s, dp;
 #pragma unroll
-            for (int i = 0; i < SP; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) { s[i][r] = 0.0f; dp[i][r] = -delta; }
-                dot_channels<DP, PT>(s[i], ki, c0 + 32 * i, qf);
-                dot_channels<DP, PT>(dp[i], vi, c0 + 32 * i, dof);
-            }
-            if (side != BIAS_NEAR && js + 32 * SP <= end && !(p.causal && hi > 0)) {
+            for (int r = 0; r < 16; ++r) { s[r] = 0.0f; dp[r] = minus_delta; }
+            dot_channels<DP, PT>(s, ki, c0, qf);
+            dot_channels<DP, PT>(dp, vi, c0, dof);
+            if (side != BIAS_NEAR && js + 32 <= end && !(p.causal && hi > 0)) {
                 const float shift = bias_flat(tab, p, side) - lse2;
 #pragma unroll
-                for (int i = 0; i < SP; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) dp[i][r] *= exp2_hw(fmaf(s[i][r], p.c, shift));
+                for (int r = 0; r < 16; ++r) dp[r] *= exp2_hw(fmaf(s[r], p.c, shift));
             } else {
                 const int stop = (p.causal ? min(end, pos + 1) : end) - js;
                 const float flat = bias_flat(tab, p, side);
 #pragma unroll
-                for (int i = 0; i < SP; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = 32 * i + acc_row(r, h);
-                        const float bias = side == BIAS_NEAR ? tab[clampi(js + row - pos, -p.far_, p.far_) + p.far_] : flat;
-                        dp[i][r] *= exp2_hw(fmaf(s[i][r], p.c, bias - lse2));
-                        if (row >= stop) dp[i][r] = 0.0f;
-                    }
+                for (int r = 0; r < 16; ++r) {
+                    const int row = acc_row(r, h);
+                    const float bias = side == BIAS_NEAR ? tab[clampi(js + row - pos, -p.far_, p.far_) + p.far_] : flat;
+                    dp[r] *= exp2_hw(fmaf(s[r], p.c, bias - lse2));
+                    if (row >= stop) dp[r] = 0.0f;
+                }
             }
             if (side == BIAS_NEAR) {
+                // transposed through LDS so that a lane owns one diagonal of the block
 #pragma unroll
-                for (int i = 0; i < SP; ++i) {
-                    // transposed through LDS so that a lane owns one diagonal of the block
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) blk_ds[acc_row(r, h) * DGP + (l & 31)] = dp[i][r];
-                    wave_lds_fence();
-                    const int dg = l - 31;                      // key index - query index
-                    float sum = 0.0f;
-                    if (l < 63) {
-                        const int i0 = dg < 0 ? -dg : 0, i1 = dg > 0 ? 32 - dg : 32;
-                        for (int e = i0; e < i1; ++e) sum += blk_ds[(e + dg) * DGP + e];
-                    }
-                    const int off = js + 32 * i - pos0 + dg;
-                    // offsets beyond the table all fall on its ends: those lanes keep their sum to themselves
-                    if (l < 63) {
-                        if (off <= -p.far_) far_left += sum;
-                        else if (off >= p.far_) far_right += sum;
-                        else hist[off + p.far_] += sum;
-                    }
-                    wave_lds_fence();
+                for (int r = 0; r < 16; ++r) blk_ds[acc_row(r, h) * DGP + (l & 31)] = dp[r] * near_fix;
+                wave_lds_fence();
+                const int dg = l - 31;                          // key index - query index
+                float sum = 0.0f;
+                if (l < 63) {
+                    const int i0 = dg < 0 ? -dg : 0, i1 = dg > 0 ? 32 - dg : 32;
+                    for (int e = i0; e < i1; ++e) sum += blk_ds[(e + dg) * DGP + e];
                 }
+                const int o = js - pos0 + dg;
+                // offsets beyond the table all fall on its ends
+                if (l < 63) {
+                    if (o <= -p.far_) end_left += sum;
+                    else if (o >= p.far_) end_right += sum;
+                    else hist[o + p.far_] += sum;
+                }
+                wave_lds_fence();
             } else if (side != BIAS_NONE) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < SP; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum += dp[i][r];
+                for (int r = 0; r < 16; ++r) sum += dp[r];
                 if (side == BIAS_LEFT) far_left += sum; else far_right += sum;
             }
-#pragma unroll
-            for (int i = 0; i < SP; ++i) dot_positions<DP, PT>(acc, ki, c0 + 32 * i, dp[i]);
+            dot_positions<DP, PT>(acc, ki, c0, dp);
         }
     }
 
@@ -200,10 +208,17 @@ void bucket_dq_kernel(Dev p)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * blk + acc_row(r, h);
-                if (d < p.head_dim) dqg[(int64_t)d * p.dqc] = (T)(valid ? acc[blk][r] * p.scale : 0.0f);
+                if (d < p.head_dim) dqg[(int64_t)d * p.dqc] = (T)(valid ? acc[blk][r] * (sgn * p.scale) : 0.0f);
             }
     }
     if (p.bias) {
+        if (lse2 < __builtin_inff()) {                      // what the rounding of (bias - lse2) and of lse2 left out
+            const float left = tab[0] - lse2, right = tab[2 * p.far_] - lse2;
+            far_left *= 1.0 + (((double)tab[0] - (double)lse2 - (double)left) - off) * (double)LN2;
+            far_right *= 1.0 + (((double)tab[2 * p.far_] - (double)lse2 - (double)right) - off) * (double)LN2;
+        }
+        far_left = (double)sgn * far_left + end_left;
+        far_right = (double)sgn * far_right + end_right;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) { far_left += __shfl_xor(far_left, o); far_right += __shfl_xor(far_right, o); }
         wave_lds_fence();
@@ -220,46 +235,45 @@ void bucket_dq_kernel(Dev p)
 // are untransposed here (rows = queries, columns = keys): a key is a lane.
 //
 // KW = 2: half of the waves take the first, half the second 32 queries of every tile (64 keys per workgroup).
-// The last workgroups of the launch do the sums of the bias gradient.
-__device__ void dbias_of_head(const Dev& p, int head, unsigned char* lds);
-
-template <typename T, int DP, int KW>
-__global__ __launch_bounds__(NTHR, (Shape<T, DP, KW>::MIN_WAVES))
-void bucket_dkv_kernel(Dev p)
+// DK, DV: which of the two this workgroup computes.
+template <typename T, int DP, int KW, bool DK, bool DV>
+__device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* lds, bool reverse = false)
 {
     using F = typename Num<T>::frag;
     using S = Shape<T, DP, KW>;
-    constexpr int KT = S::KT, NS = S::NS, SP = S::SP, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, CW = NWAVE / KW;
-    extern __shared__ __align__(16) unsigned char lds[];
-    if ((int)blockIdx.x >= p.kv_blocks) { dbias_of_head(p, (int)blockIdx.x - p.kv_blocks, lds); return; }
+    constexpr int KT = S::KT_DKV, NS = KT / 32 / KW, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, CW = NWAVE / KW;
     T* qim = reinterpret_cast<T*>(lds);
-    T* dim = qim + DP * PT;
-    float* st = reinterpret_cast<float*>(dim + DP * PT);        // log-sum-exp and delta of the tile's queries
+    T* dim = reinterpret_cast<T*>(lds + S::OWN);
+    float* st = reinterpret_cast<float*>(lds + S::IMAGES);      // log-sum-exp and -delta of the tile's queries
     float* tab = st + 2 * KT;
 
-    const Place at = place(p);
+    const Place at = place(p, id);
     if (!at.any) return;
     const int b = at.b, kvh = at.kvh;
-    const Item it = item_of(p, b);
+    const Item it = uniform_item(p, b);
     const int l = threadIdx.x & 63, h = l >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int cw = wave / KW, kw = wave % KW;
-    const int kt0 = at.within * CW * 32, jb = kt0 + cw * 32, j = jb + (l & 31);
+    const int within = reverse ? p.per_unit - 1 - at.within : at.within;
+    const int kt0 = within * CW * 32, jb = kt0 + cw * 32, j = jb + (l & 31);
     const bool valid = j < it.nk;
+    const int64_t hd = (int64_t)kvh * p.head_dim;
 
-    F kf[DP / KS], vf[DP / KS];
+    F kf[DP / KS], vf[DK ? DP / KS : 1];
     if (kt0 < it.nk) {
-        OwnRows<T, DP, KT, CW> rk, rv;
-        const int64_t hd = (int64_t)kvh * p.head_dim;
+        OwnRows<T, DP, 64, CW> rk, rv;
         rk.load((const T*)p.k + (int64_t)b * p.kb + hd * p.kc, p.kc, p.head_dim, kt0, it.nk);
-        rv.load((const T*)p.v + (int64_t)b * p.vb + hd * p.vc, p.vc, p.head_dim, kt0, it.nk);
+        if constexpr (DK) rv.load((const T*)p.v + (int64_t)b * p.vb + hd * p.vc, p.vc, p.head_dim, kt0, it.nk);
         rk.frags(kf, qim, dim, cw);
-        rv.frags(vf, qim, dim, cw);
+        if constexpr (DK) rv.frags(vf, qim, dim, cw);
     }
-    f32x16 dk[DP / 32], dv[DP / 32];
+    f32x16 dk[DK ? DP / 32 : 1], dv[DV ? DP / 32 : 1];
 #pragma unroll
     for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { dk[blk][r] = 0.0f; dv[blk][r] = 0.0f; }
+        for (int r = 0; r < 16; ++r) {
+            if constexpr (DK) dk[blk][r] = 0.0f;
+            if constexpr (DV) dv[blk][r] = 0.0f;
+        }
 
     // queries that see any of these keys: with `causal` those at or behind the first key
     int q_first = 0;
@@ -272,72 +286,61 @@ void bucket_dkv_kernel(Dev p)
     auto fetch = [&](int step) {
         const int g = step / tiles, i0 = q_first + (step - g * tiles) * KT;
         const int head = kvh * p.group + g;
-        const int64_t hd = (int64_t)head * p.head_dim;
-        qt.load((const T*)p.q + (int64_t)b * p.qb + hd * p.qc, p.qc, p.head_dim, i0, it.nq);
-        dt.load((const T*)p.dout + (int64_t)b * p.dob + hd * p.doc, p.doc, p.head_dim, i0, it.nq);
+        qt.load((const T*)p.q + (int64_t)b * p.qb + (int64_t)head * p.head_dim * p.qc, p.qc, p.head_dim, i0, it.nq);
+        dt.load((const T*)p.dout + (int64_t)b * p.dob + (int64_t)head * p.head_dim * p.doc, p.doc, p.head_dim, i0, it.nq);
         const int64_t row = ((int64_t)b * p.heads + head) * p.queries;
         const int i = i0 + ((int)threadIdx.x & (KT - 1));
-        if (threadIdx.x < KT) {
-            stat = __builtin_inff();
-            if (i < it.nq) { const float v = p.lse_in[row + i]; stat = v == -__builtin_inff() ? __builtin_inff() : v * LOG2E; }
-        } else if (threadIdx.x < 2 * KT) {
-            stat = i < it.nq ? p.delta[row + i] : 0.0f;
+        if (threadIdx.x < 2 * KT) {                 // converted when it is stored: using it here would wait for all loads
+            const float* src = threadIdx.x < KT ? p.lse_in : p.delta;
+            stat = i < it.nq ? src[row + i] : threadIdx.x < KT ? -__builtin_inff() : 0.0f;
         }
     };
-    if (steps > 0) fetch(0);
+    if (S::AHEAD && steps > 0) fetch(0);
     for (int step = 0; step < steps; ++step) {
         const int g = step / tiles, tile = step - g * tiles, i0 = q_first + tile * KT;
+        if constexpr (!S::AHEAD) fetch(step);
         __syncthreads();
         qt.store(qim);
         dt.store(dim);
-        if (threadIdx.x < 2 * KT) st[threadIdx.x] = stat;
+        if (threadIdx.x < KT) st[threadIdx.x] = stat == -__builtin_inff() ? __builtin_inff() : stat * LOG2E;    // no keys: all probabilities 0
+        else if (threadIdx.x < 2 * KT) st[threadIdx.x] = -stat;
         if (tile == 0) stage_bias(tab, p, kvh * p.group + g);
         __syncthreads();
-        if (step + 1 < steps) fetch(step + 1);
+        if (S::AHEAD && step + 1 < steps) fetch(step + 1);
 #pragma unroll
-        for (int sp = 0; sp < NS / SP; ++sp) {
-            const int c0 = 32 * (kw * NS + sp * SP), is = i0 + c0, pos0 = it.start + is;      // this step's queries
-            if (is >= it.nq || (p.causal && jb > pos0 + 32 * SP - 1)) continue;
-            const int lo = jb - (pos0 + 32 * SP - 1), hi = jb + 31 - pos0, side = bias_side(p, lo, hi);
-            f32x16 s[SP], dp[SP];
+        for (int i = 0; i < NS; ++i) {
+            const int c0 = 32 * (kw * NS + i), is = i0 + c0, pos0 = it.start + is;     // this block's queries
+            if (is >= it.nq || (p.causal && jb > pos0 + 31)) continue;
+            const int lo = jb - (pos0 + 31), hi = jb + 31 - pos0, side = bias_side(p, lo, hi);
+            f32x16 s, dp;
 #pragma unroll
-            for (int i = 0; i < SP; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) { s[i][r] = 0.0f; dp[i][r] = -st[KT + c0 + 32 * i + acc_row(r, h)]; }
-                dot_channels<DP, PT>(s[i], qim, c0 + 32 * i, kf);
-                dot_channels<DP, PT>(dp[i], dim, c0 + 32 * i, vf);
-            }
+            for (int r = 0; r < 16; ++r) { s[r] = 0.0f; if constexpr (DK) dp[r] = st[KT + c0 + acc_row(r, h)]; }
+            dot_channels<DP, PT>(s, qim, c0, kf);
+            if constexpr (DK) dot_channels<DP, PT>(dp, dim, c0, vf);
             const float flat = bias_flat(tab, p, side);
             if (side != BIAS_NEAR && !(p.causal && hi > 0)) {
 #pragma unroll
-                for (int i = 0; i < SP; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        s[i][r] = exp2_hw(fmaf(s[i][r], p.c, flat - st[c0 + 32 * i + acc_row(r, h)]));
+                for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], p.c, flat - st[c0 + acc_row(r, h)]));
             } else {
 #pragma unroll
-                for (int i = 0; i < SP; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int row = 32 * i + acc_row(r, h), off = j - (pos0 + row);
-                        const float bias = side == BIAS_NEAR ? tab[clampi(off, -p.far_, p.far_) + p.far_] : flat;
-                        s[i][r] = exp2_hw(fmaf(s[i][r], p.c, bias - st[c0 + row]));
-                        if (p.causal && off > 0) s[i][r] = 0.0f;
-                    }
+                for (int r = 0; r < 16; ++r) {
+                    const int row = acc_row(r, h), off = j - (pos0 + row);
+                    const float bias = side == BIAS_NEAR ? tab[clampi(off, -p.far_, p.far_) + p.far_] : flat;
+                    s[r] = exp2_hw(fmaf(s[r], p.c, bias - st[c0 + row]));
+                    if (p.causal && off > 0) s[r] = 0.0f;
+                }
             }
+            if constexpr (DV) dot_positions<DP, PT>(dv, dim, c0, s);
+            if constexpr (DK) {
 #pragma unroll
-            for (int i = 0; i < SP; ++i) dot_positions<DP, PT>(dv, dim, c0 + 32 * i, s[i]);
-#pragma unroll
-            for (int i = 0; i < SP; ++i) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[i][r] *= dp[i][r];
-                dot_positions<DP, PT>(dk, qim, c0 + 32 * i, s[i]);
+                for (int r = 0; r < 16; ++r) s[r] *= dp[r];
+                dot_positions<DP, PT>(dk, qim, c0, s);
             }
         }
     }
-    if constexpr (KW == 2) {
-        float* red = reinterpret_cast<float*>(lds) + cw * DP * 32 + (l & 31);
-        auto join = [&](f32x16 (&x)[DP / 32]) {
+    float* red = reinterpret_cast<float*>(lds) + cw * DP * 32 + (l & 31);
+    auto finish = [&](f32x16 (&x)[DP / 32], void* out, int64_t bstride, int64_t cstride, float scale) {
+        if constexpr (KW == 2) {
             __syncthreads();
             if (kw == 1)
 #pragma unroll
@@ -350,30 +353,24 @@ void bucket_dkv_kernel(Dev p)
                 for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) x[blk][r] += red[(32 * blk + acc_row(r, h)) * 32];
-        };
-        join(dk);
-        join(dv);
-    }
-    if (j < p.keys && kw == 0) {
-        const int64_t hd = (int64_t)kvh * p.head_dim;
-        T* dkg = (T*)p.dk + (int64_t)b * p.dkb + hd * p.dkc + j;
-        T* dvg = (T*)p.dv + (int64_t)b * p.dvb + hd * p.dvc + j;
+        }
+        if (j >= p.keys || kw != 0) return;
+        T* g = (T*)out + (int64_t)b * bstride + hd * cstride + j;
 #pragma unroll
         for (int blk = 0; blk < DP / 32; ++blk)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int d = 32 * blk + acc_row(r, h);
-                if (d < p.head_dim) {
-                    dkg[(int64_t)d * p.dkc] = (T)(valid ? dk[blk][r] * p.scale : 0.0f);
-                    dvg[(int64_t)d * p.dvc] = (T)(valid ? dv[blk][r] : 0.0f);
-                }
+                if (d < p.head_dim) g[(int64_t)d * cstride] = (T)(valid ? x[blk][r] * scale : 0.0f);
             }
-    }
+    };
+    if constexpr (DK) finish(dk, p.dk, p.dkb, p.dkc, p.scale);
+    if constexpr (DV) finish(dv, p.dv, p.dvb, p.dvc, 1.0f);
 }
 
 // dbias[h, c] = sum of the diagonal sums whose offset falls into bucket c, over all workgroups of head h, in 64 bits
 // (the sums of a row cancel to zero).
-__device__ void dbias_of_head(const Dev& p, int head, unsigned char* lds)
+__device__ __forceinline__ void dbias_of_head(const Dev& p, int head, unsigned char* lds)
 {
     const int offsets = 2 * p.far_ + 1, tid = (int)threadIdx.x, parts = p.batch * p.tiles;
     float* sums = reinterpret_cast<float*>(lds);
@@ -404,16 +401,34 @@ __device__ void dbias_of_head(const Dev& p, int head, unsigned char* lds)
     }
 }
 
+// The gradients of keys and values; the last workgroups of the launch do the sums of the bias gradient.
+template <typename T, int DP, int KW>
+__global__ __launch_bounds__(NTHR, (Shape<T, DP, KW>::MIN_WAVES))
+void bucket_dkv_kernel(Dev p)
+{
+    extern __shared__ __align__(16) unsigned char lds[];
+    int id = (int)blockIdx.x;
+    if constexpr (Shape<T, DP, KW>::SPLIT) {
+        if (id < p.kv_blocks) return key_side<T, DP, KW, true, false>(p, id, lds);
+        id -= p.kv_blocks;
+        if (id < p.kv_blocks) return key_side<T, DP, KW, false, true>(p, id, lds, p.fold);
+    } else {
+        if (id < p.kv_blocks) return key_side<T, DP, KW, true, true>(p, id, lds);
+    }
+    dbias_of_head(p, id - p.kv_blocks, lds);
+}
+
 template <typename T, int DP, int KW>
 int launch_both(Dev d, hipStream_t st)
 {
-    const size_t img = 2 * (size_t)Tile<T, DP, Shape<T, DP, KW>::KT>::BYTES, offsets = 2 * (size_t)d.far_ + 1;
+    using S = Shape<T, DP, KW>;
+    const size_t offsets = 2 * (size_t)d.far_ + 1;
     const char* what = "vk_bucket_attention_backward";
     constexpr int ROWS = NWAVE / KW * 32;
     d.tiles = (d.queries + ROWS - 1) / ROWS;
     if (d.queries > 0) {
         vkba_place(d, (int64_t)d.tiles * d.group);
-        const size_t lds = img + vkba_table_bytes(d) + (d.bias ? NWAVE * (offsets + 32 * DGP) * 4 : 0);
+        const size_t lds = S::IMAGES + vkba_table_bytes(d) + (d.bias ? NWAVE * (offsets + 32 * DGP) * 4 : 0);
         int rc = vkba_launch<bucket_dq_kernel<T, DP, KW>>(d, vkba_blocks(d), lds, st, what);
         if (rc != VK_OK) return rc;
     }
@@ -421,8 +436,12 @@ int launch_both(Dev d, hipStream_t st)
     const int64_t blocks = d.keys > 0 ? vkba_blocks(d) : 0;
     if (blocks > 0x7fffffff) return vkba_fail(VK_E_UNSUPPORTED, what, "too many workgroups");
     d.kv_blocks = (int)blocks;
-    const size_t need = img + 2 * Shape<T, DP, KW>::KT * 4 + vkba_table_bytes(d);
-    return vkba_launch<bucket_dkv_kernel<T, DP, KW>>(d, blocks + (d.bias ? d.heads : 0), need > offsets * 8 ? need : offsets * 8, st, what);
+    // causal: the first keys have the most queries.  Where all workgroups find a place at once (two on every CU),
+    // those of dv come in the other order, so that a CU gets a long and a short one
+    d.fold = d.causal && 2 * blocks <= 512;
+    const size_t need = S::IMAGES + 2 * S::KT_DKV * 4 + vkba_table_bytes(d);
+    return vkba_launch<bucket_dkv_kernel<T, DP, KW>>(d, (S::SPLIT ? 2 : 1) * blocks + (d.bias ? d.heads : 0),
+                                                     need > offsets * 8 ? need : offsets * 8, st, what);
 }
 
 template <typename T, int KW>
@@ -436,13 +455,10 @@ int by_width(const Dev& d, hipStream_t st)
     }
 }
 
-#ifndef KWB
-#define KWB 256
-#endif
 // Rows (queries of the first, keys of the second kernel) per workgroup.
 int key_waves(const vk_bucket_attention_args* a)
 {
-    return a->dtype == VK_DTYPE_F32 || (int64_t)a->batch * a->heads * ((a->queries + 127) / 128) < KWB ? 2 : 1;
+    return a->dtype == VK_DTYPE_F32 || (int64_t)a->batch * a->heads * ((a->queries + 127) / 128) < 256 ? 2 : 1;
 }
 int64_t parts_of_head(const vk_bucket_attention_args* a)
 {

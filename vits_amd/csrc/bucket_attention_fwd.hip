@@ -17,31 +17,28 @@ constexpr int FWD_TILE = 64;    // keys of a staged tile
 // instead of 128), each with a maximum, sum and output of its own, joined through LDS at the end.  The staging of
 // a tile is then shared by half the work, but there are twice the workgroups.
 template <typename T, int DP, int KW>
-#ifndef BW64
-#define BW64 3
-#endif
-#ifndef FW
-#define FW 2
-#endif
-__global__ __launch_bounds__(NTHR, sizeof(T) == 4 ? FW : (DP <= 64 ? BW64 : 2))
+__global__ __launch_bounds__(NTHR, (sizeof(T) == 2 && DP <= 64 ? 3 : 2))
 void bucket_attention_kernel(Dev p)
 {
     using F = typename Num<T>::frag;
     constexpr int KT = FWD_TILE, KS = Num<T>::KS, PT = Tile<T, DP, KT>::PT, QW = NWAVE / KW, QT = QW * 32;
     constexpr int NS = KT / 32 / KW;                              // 32-key blocks of a tile per wave
+    // the next tile is loaded into registers while the present one is computed; in fp32, where a tile takes four times
+    // the matrix cycles, those registers are worth more as a second wave per SIMD
+    constexpr bool AHEAD = sizeof(T) == 2;
     constexpr int SP = sizeof(T) == 4 ? 1 : NS;             // of them in one softmax step (fp32: 1, to keep the registers)
     extern __shared__ __align__(16) unsigned char lds[];
     T* ki = reinterpret_cast<T*>(lds);
     T* vi = ki + DP * PT;
     float* tab = reinterpret_cast<float*>(vi + DP * PT);
 
-    const Place at = place(p);
+    const Place at = place(p, (int)blockIdx.x);
     if (!at.any) return;
     const int b = at.b, kvh = at.kvh, g = at.within % p.group, rest = at.within / p.group;
     const int split = rest % p.splits;
     const int qt = p.tiles - 1 - rest / p.splits;           // causal: the longest rows first
     const int head = kvh * p.group + g;
-    const Item it = item_of(p, b);
+    const Item it = uniform_item(p, b);
     const int l = threadIdx.x & 63, h = l >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int qw = wave / KW, kw = wave % KW;
     const int q0 = qt * QT + qw * 32, qi = q0 + (l & 31);
@@ -62,8 +59,10 @@ void bucket_attention_kernel(Dev p)
     if (first < end) {
         OwnRows<T, DP, KT, QW> rows;
         rows.load((const T*)p.q + (int64_t)b * p.qb + (int64_t)head * p.head_dim * p.qc, p.qc, p.head_dim, qt * QT, it.nq);
-        kt.load(kg, p.kc, p.head_dim, first, end);
-        vt.load(vg, p.vc, p.head_dim, first, end);
+        if constexpr (AHEAD) {
+            kt.load(kg, p.kc, p.head_dim, first, end);
+            vt.load(vg, p.vc, p.head_dim, first, end);
+        }
         stage_bias(tab, p, head);
         rows.frags(qf, ki, vi, qw);
     }
@@ -78,11 +77,15 @@ void bucket_attention_kernel(Dev p)
     const float c = p.c;
     const int pos0 = it.start + q0, pos = pos0 + (l & 31);
     for (int j0 = first; j0 < end; j0 += KT) {
+        if constexpr (!AHEAD) {
+            kt.load(kg, p.kc, p.head_dim, j0, end);
+            vt.load(vg, p.vc, p.head_dim, j0, end);
+        }
         __syncthreads();
         kt.store(ki);
         vt.store(vi);
         __syncthreads();
-        if (j0 + KT < end) {
+        if (AHEAD && j0 + KT < end) {
             kt.load(kg, p.kc, p.head_dim, j0 + KT, end);
             vt.load(vg, p.vc, p.head_dim, j0 + KT, end);
         }
@@ -262,20 +265,14 @@ int by_width(const Dev& d, int kw, hipStream_t st)
 }
 
 // Queries per workgroup (128 or, with the waves in two key halves, 64) and shares of the keys' length.
-#ifndef KWB
-#define KWB 256
-#endif
-#ifndef SPB
-#define SPB 256
-#endif
 void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& kw)
 {
     const int64_t heads = (int64_t)a->batch * a->heads;
-    kw = a->dtype == VK_DTYPE_F32 || heads * ((a->queries + 127) / 128) < KWB ? 2 : 1;
+    kw = a->dtype == VK_DTYPE_F32 || heads * ((a->queries + 127) / 128) < 256 ? 2 : 1;
     d.tiles = (a->queries + 128 / kw - 1) / (128 / kw);
     const int64_t blocks = heads * d.tiles;
     const int key_tiles = (a->keys + FWD_TILE - 1) / FWD_TILE;
-    int64_t splits = blocks >= SPB || blocks == 0 ? 1 : (2 * SPB + blocks - 1) / blocks;
+    int64_t splits = blocks >= 256 || blocks == 0 ? 1 : (512 + blocks - 1) / blocks;
     splits = splits > (key_tiles + 1) / 2 ? (key_tiles + 1) / 2 : splits;
     if (splits < 1) splits = 1;
     d.per_split = (int)((key_tiles + splits - 1) / splits);
