@@ -59,24 +59,27 @@ class RelativeBuckets:
     def table(self, device) -> torch.Tensor:
         """int32 [2 * max_distance + 1] on ``device``: the bucket of every offset from -max_distance up.
         Made once per device."""
-        key = native._device_index(device)
-        t = self._tables.get(key)
+        device = torch.device(device)
+        t = self._tables.get(device.index)
         if t is None:
+            key = native._device_index(device)
             if torch.cuda.is_current_stream_capturing():
                 raise native.NativeError("call RelativeBuckets.table(device) before the capture")
             t = torch.tensor([self.bucket_of(o) for o in range(-self.max_distance, self.max_distance + 1)],
                              dtype=torch.int32).to(torch.device("cuda", key))
-            self._tables[key] = t
+            self._tables[key] = self._tables[device.index] = t
         return t
 
 
 def _view3(name, t, dtype, device, shape=None):
+    if t.dtype is dtype and t.device == device and t.dim() == 3 and (shape is None or t.shape == shape) \
+            and (t.stride(2) == 1 or t.shape[2] <= 1):
+        return
     if t.dim() != 3 or t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be [batch, channels, time] of {dtype} on {device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
-        raise ValueError(f"{name} must have a dense time axis, strides are {t.stride()}")
+    raise ValueError(f"{name} must have a dense time axis, strides are {t.stride()}")
 
 
 def _lengths(name, t, batch, device):
@@ -88,29 +91,32 @@ def _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, 
     """Checks what both passes take; returns (kv_heads, scale, bucket table or None)."""
     if not q.is_cuda:
         raise native.NativeError("bucket_attention runs on the GPU only: there is no CPU fallback")
-    if q.dtype not in native.DTYPES:
-        raise ValueError(f"q must be float32 or bfloat16, got {q.dtype}")
+    dtype, device = q.dtype, q.device
+    if dtype not in native.DTYPES:
+        raise ValueError(f"q must be float32 or bfloat16, got {dtype}")
     kv_heads = heads if kv_heads is None else kv_heads
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"heads ({heads}) must be a multiple of kv_heads ({kv_heads})")
-    _view3("q", q, q.dtype, q.device)
+    _view3("q", q, dtype, device)
     B, C, _ = q.shape
     if C % heads or not 1 <= C // heads <= native.BUCKET_MAX_HEAD_DIM:
         raise ValueError(f"q's {C} channels are not {heads} heads of 1..{native.BUCKET_MAX_HEAD_DIM}")
-    _view3("k", k, q.dtype, q.device)
-    _view3("k", k, q.dtype, q.device, (B, C // heads * kv_heads, k.shape[2]))
-    _view3("v", v, q.dtype, q.device, k.shape)
-    _lengths("key_lengths", key_lengths, B, q.device)
-    _lengths("query_lengths", query_lengths, B, q.device)
-    _lengths("query_start", query_start, B, q.device)
+    _view3("k", k, dtype, device)
+    shape = k.shape
+    if shape[0] != B or shape[1] != C // heads * kv_heads:
+        raise ValueError(f"k must be {(B, C // heads * kv_heads, shape[2])}, got {tuple(shape)}")
+    _view3("v", v, dtype, device, shape)
+    _lengths("key_lengths", key_lengths, B, device)
+    _lengths("query_lengths", query_lengths, B, device)
+    _lengths("query_start", query_start, B, device)
     table = None
     if (bias is None) != (buckets is None):
         raise ValueError("bias and buckets go together")
     if bias is not None:
-        if bias.dtype != torch.float32 or bias.device != q.device or tuple(bias.shape) != (heads, buckets.num_buckets) \
+        if bias.dtype is not torch.float32 or bias.device != device or bias.shape != (heads, buckets.num_buckets) \
                 or not bias.is_contiguous():
-            raise ValueError(f"bias must be a contiguous float32 [{heads}, {buckets.num_buckets}] on {q.device}")
-        table = buckets.table(q.device)
+            raise ValueError(f"bias must be a contiguous float32 [{heads}, {buckets.num_buckets}] on {device}")
+        table = buckets.table(device)
     scale = (C // heads) ** -0.5 if scale is None else float(scale)
     if not 0 < scale < 1e30:
         raise ValueError("scale must be positive and finite")
@@ -118,8 +124,8 @@ def _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, 
 
 
 def _forward(q, k, v, bias, table, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty((q.shape[0], heads, q.shape[2]), device=q.device, dtype=torch.float32)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((q.shape[0], heads, q.shape[2]), dtype=torch.float32)
     native.bucket_attention(q, k, v, out, lse, bias, table, heads=heads, kv_heads=kv_heads, key_lengths=key_lengths,
                             query_lengths=query_lengths, query_start=query_start, causal=causal, scale=scale)
     return out, lse
@@ -128,8 +134,8 @@ def _forward(q, k, v, bias, table, heads, kv_heads, key_lengths, query_lengths, 
 def _backward(dout, q, k, v, out, lse, bias, table, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
     if dout.stride(2) != 1 and dout.shape[2] > 1:           # gradients of sums come expanded
         dout = dout.contiguous()
-    dq, dk, dv = (torch.empty(t.shape, device=q.device, dtype=q.dtype) for t in (q, k, v))
-    dbias = torch.empty(bias.shape, device=q.device, dtype=torch.float32) if bias is not None else None
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dbias = torch.empty_like(bias) if bias is not None else None
     native.bucket_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, bias, table, dbias, heads=heads, kv_heads=kv_heads,
                                      key_lengths=key_lengths, query_lengths=query_lengths, query_start=query_start,
                                      causal=causal, scale=scale)

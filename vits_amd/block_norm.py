@@ -38,8 +38,8 @@ def _dense(t):
 
 
 def _param(name, t, channels, device):
-    if t is not None and (t.dtype != torch.float32 or t.device != device or tuple(t.shape) != (channels,) or not t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous float32 [{channels}] on {device}")
+    if t is not None and (t.dtype is not torch.float32 or t.device != device or t.shape != (channels,) or not t.is_contiguous()):
+        raise ValueError(f"{name} (or its weight or bias) must be a contiguous float32 [{channels}] on {device}")
 
 
 def _check(like, y, gate, scale, post, pre, norm, eps, lengths):
@@ -47,39 +47,40 @@ def _check(like, y, gate, scale, post, pre, norm, eps, lengths):
         raise native.NativeError("block_norm runs on the GPU only: there is no CPU fallback")
     if like.dtype not in native.DTYPES:
         raise ValueError(f"x must be float32 or bfloat16, got {like.dtype}")
-    _view3("x", like, like.dtype, like.device)
-    B, C, T = like.shape
+    dtype, device = like.dtype, like.device
+    _view3("x", like, dtype, device)
+    shape = like.shape
+    B, C, T = shape
     if not 1 <= C <= native.BLOCK_NORM_MAX_CHANNELS:
         raise ValueError(f"channels must be 1..{native.BLOCK_NORM_MAX_CHANNELS}, got {C}")
     if y is None:
         if gate is not None or scale is not None or post is not None:
             raise ValueError("gate, scale and post go with y")
     else:
-        _view3("y", y, like.dtype, like.device, like.shape)
+        _view3("y", y, dtype, device, shape)
     if gate is not None:
-        _view3("gate", gate, like.dtype, like.device)
-        if tuple(gate.shape) not in ((B, C, T), (B, C, 1)):
+        _view3("gate", gate, dtype, device)
+        if gate.shape != shape and gate.shape != (B, C, 1):
             raise ValueError(f"gate must be {(B, C, T)} or {(B, C, 1)}, got {tuple(gate.shape)}")
-    _param("scale", scale, C, like.device)
+    _param("scale", scale, C, device)
     for name, pair in (("post", post), ("pre", pre)):
         if pair is not None:
             if pair[0] is None:
                 raise ValueError(f"{name} is (weight, bias or None)")
-            _param(name + " weight", pair[0], C, like.device)
-            _param(name + " bias", pair[1], C, like.device)
+            _param(name, pair[0], C, device)
+            _param(name, pair[1], C, device)
     if norm not in _NORMS:
         raise ValueError(f"norm must be one of {sorted(_NORMS)}")
     if not 0 < eps < 1e30:
         raise ValueError("eps must be positive and finite")
     if y is None and pre is None:
         raise ValueError("nothing to do: neither y nor pre is given")
-    _lengths("lengths", lengths, B, like.device)
+    _lengths("lengths", lengths, B, device)
 
 
 def _forward(x, y, gate, scale, post, pre, norm, eps, lengths):
-    new = lambda: torch.empty(x.shape, device=x.device, dtype=x.dtype)  # noqa: E731
-    h = new() if y is not None else None
-    n = new() if pre is not None else None
+    h = x.new_empty(x.shape) if y is not None else None
+    n = x.new_empty(x.shape) if pre is not None else None
     native.block_norm(x, y, h, n, gate=gate, scale=scale, post=post, pre=pre, norm=_NORMS[norm], eps=eps, lengths=lengths)
     return h, n
 
@@ -87,7 +88,7 @@ def _forward(x, y, gate, scale, post, pre, norm, eps, lengths):
 def _backward(dh, dn, h, y, gate, scale, post, pre, norm, eps, lengths):
     dh, dn = _dense(dh), _dense(dn)
     like = dh if dh is not None else dn
-    new = lambda t: torch.empty(t.shape, device=like.device, dtype=like.dtype) if t is not None else None  # noqa: E731
+    new = lambda t: t.new_empty(t.shape) if t is not None else None  # noqa: E731
     par = lambda t: torch.empty_like(t) if t is not None else None  # noqa: E731
     dx, dy, dgate, dscale = new(like), new(y), new(gate), par(scale)
     dpost = (par(post[0]), par(post[1])) if post is not None else None

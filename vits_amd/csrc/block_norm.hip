@@ -16,10 +16,11 @@
 #include <string.h>
 #include "../../include/vits_amd.h"
 #include "api_internal.hpp"
+#include "chunk_load.hpp"
 
 namespace {
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef chunk_t u32x4;
 
 struct NDev {
     vk_block_norm_args a;
@@ -30,23 +31,6 @@ struct NDev {
 
 template <typename T> struct Pack { static constexpr int E = 16 / (int)sizeof(T); };
 
-// 16 bytes of a row from position t; columns at or behind `limit` are 0 and not read.  Rows of odd length start
-// anywhere, so the access is declared unaligned.
-template <typename T>
-__device__ __forceinline__ u32x4 load_raw(const T* row, int t, int limit)
-{
-    constexpr int E = Pack<T>::E;
-    u32x4 r = {0u, 0u, 0u, 0u};
-    if (t + E <= limit) {
-        __builtin_memcpy(&r, row + t, 16);
-    } else if (t < limit) {
-        T tmp[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) tmp[e] = t + e < limit ? row[t + e] : (T)0.0f;
-        __builtin_memcpy(&r, tmp, 16);
-    }
-    return r;
-}
 __device__ __forceinline__ void unpack(float (&v)[4], const u32x4& r)
 {
 #pragma unroll
@@ -140,7 +124,7 @@ __device__ __forceinline__ void column_stats(F value, int rows, int channels, fl
 template <typename T, int LT, int NW>
 struct Spot {
     static constexpr int E = Pack<T>::E, CG = 64 / LT * NW;
-    int cg, rows, b, t, live, lt;
+    int cg, rows, b, t, live, lt, channels;
     __device__ __forceinline__ Spot(const NDev& p)
     {
         const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
@@ -148,6 +132,7 @@ struct Spot {
         cg = wave * (64 / LT) + lane / LT;
         b = (int)blockIdx.x / p.windows;
         t = ((int)blockIdx.x - b * p.windows) * LT * E + lt * E;
+        channels = p.a.channels;
         live = p.a.length;
         if (p.a.lengths) { const int64_t n = p.a.lengths[b]; live = (int)(n < 0 ? 0 : n > p.a.length ? p.a.length : n); }
         rows = cg < p.a.channels ? (p.a.channels - cg + CG - 1) / CG : 0;
@@ -156,9 +141,10 @@ struct Spot {
     template <int R>
     __device__ __forceinline__ void load(u32x4 (&v)[R], const void* base, int64_t bstride, int64_t cstride) const
     {
-        const T* p = (const T*)base + (int64_t)b * bstride + (int64_t)cg * cstride;
+        // threads without a channel read the last one again: the loads stay free of branches
+        const T* p = (const T*)base + (int64_t)b * bstride;
 #pragma unroll
-        for (int r = 0; r < R; ++r) v[r] = r < rows ? load_raw<T>(p + (int64_t)(r * CG) * cstride, t, live) : u32x4{0u, 0u, 0u, 0u};
+        for (int r = 0; r < R; ++r) v[r] = load_chunk<T>(p + (int64_t)min(channel(r), channels - 1) * cstride, t, live);
     }
     __device__ __forceinline__ T* row(void* base, int64_t bstride, int64_t cstride, int r) const
     {
@@ -313,7 +299,7 @@ void block_norm_backward_kernel(NDev p)
         if (r >= at.rows) continue;
         if (a.dh) {
             float d[E];
-            unpack(d, load_raw<T>((const T*)a.dh + (int64_t)at.b * a.dh_bstride + (int64_t)at.channel(r) * a.dh_cstride, at.t, at.live));
+            unpack(d, load_chunk<T>((const T*)a.dh + (int64_t)at.b * a.dh_bstride + (int64_t)at.channel(r) * a.dh_cstride, at.t, at.live));
 #pragma unroll
             for (int e = 0; e < E; ++e) g[r][e] += d[e];
         }
@@ -333,7 +319,7 @@ void block_norm_backward_kernel(NDev p)
         const float w = a.w_post ? a.w_post[c] : 1.0f, bias = a.b_post ? a.b_post[c] : 0.0f;
         float gate[E], dg[E], ds[E], dw[E], v[E];
         if (a.gate && !a.gate_per_item) {
-            unpack(gate, load_raw<T>((const T*)a.gate + (int64_t)at.b * a.gate_bstride + (int64_t)c * a.gate_cstride, at.t, at.live));
+            unpack(gate, load_chunk<T>((const T*)a.gate + (int64_t)at.b * a.gate_bstride + (int64_t)c * a.gate_cstride, at.t, at.live));
         } else {
             const float q = a.gate ? (float)((const T*)a.gate)[(int64_t)at.b * a.gate_bstride + (int64_t)c * a.gate_cstride] : 1.0f;
 #pragma unroll

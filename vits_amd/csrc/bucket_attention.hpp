@@ -24,6 +24,7 @@
 #include <stdint.h>
 #include <string.h>
 #include "../../include/vits_amd.h"
+#include "chunk_load.hpp"
 
 namespace vkba {
 
@@ -33,7 +34,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short  s16x4  __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef chunk_t u32x4;
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int NWAVE = 4;        // waves of a workgroup
@@ -53,24 +54,6 @@ __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __b
 __device__ __forceinline__ f32x16 mma(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// 16 bytes of a row at position t; positions at or behind `limit` are zero and not read.  Rows of odd
-// length start anywhere, so the load is declared unaligned (the memory system takes it as one access).
-template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T* row, int t, int limit)
-{
-    constexpr int E = Num<T>::EPC;
-    u32x4 r = {0u, 0u, 0u, 0u};
-    if (t + E <= limit) {
-        __builtin_memcpy(&r, row + t, 16);
-    } else if (t < limit) {
-        T tmp[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) tmp[e] = t + e < limit ? row[t + e] : (T)0.0f;
-        __builtin_memcpy(&r, tmp, 16);
-    }
-    return r;
-}
 
 // A [DP channels][KT positions] tile on its way from memory to its LDS image, through registers.
 template <typename T, int DP, int KT>
@@ -98,7 +81,8 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int d = row + i * ROWS;
-            c[i] = d < d_real ? load_chunk<T>(base + (int64_t)d * cstride, t0 + col, limit) : u32x4{0u, 0u, 0u, 0u};
+            const u32x4 v = load_chunk<T>(base + (int64_t)(d < d_real ? d : d_real - 1) * cstride, t0 + col, limit);
+            c[i] = d < d_real ? v : u32x4{0u, 0u, 0u, 0u};
         }
     }
     __device__ __forceinline__ void store(T* img) const

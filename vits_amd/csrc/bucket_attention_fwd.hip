@@ -5,6 +5,7 @@
 // columns = queries), so a query is a lane: its maximum and sum are lane-local but for one exchange
 // between the two lane halves, and the probabilities are already the right operand of P V.
 #include "bucket_attention.hpp"
+#include "bucket_attention_narrow.hpp"
 #include "api_internal.hpp"
 #include "bucket_attention_host.hpp"
 
@@ -264,22 +265,60 @@ int by_width(const Dev& d, int kw, hipStream_t st)
     }
 }
 
-// Queries per workgroup (128 or, with the waves in two key halves, 64) and shares of the keys' length.
+template <typename T>
+int narrow_by_width(const Dev& d, hipStream_t st)
+{
+    const char* what = "vk_bucket_attention";
+    const int heads = d.group < 16 ? d.group : 16;              // of which a tile of 16 rows can hold rows
+    const size_t tab = (size_t)heads * (2 * d.far_ + 1) * 4;
+    auto lds = [&](int dp) { const size_t red = (size_t)NWAVE * (dp + 2) * 16 * 4; return red > tab ? red : tab; };
+    switch ((d.head_dim + 31) / 32) {
+    case 1: return vkba_launch<bucket_attention_narrow_kernel<T, 32>>(d, vkba_blocks(d), lds(32), st, what);
+    case 2: return vkba_launch<bucket_attention_narrow_kernel<T, 64>>(d, vkba_blocks(d), lds(64), st, what);
+    case 3: return vkba_launch<bucket_attention_narrow_kernel<T, 96>>(d, vkba_blocks(d), lds(96), st, what);
+    default: return vkba_launch<bucket_attention_narrow_kernel<T, 128>>(d, vkba_blocks(d), lds(128), st, what);
+    }
+}
+
+#ifndef NARROW_WORK
+#define NARROW_WORK 6e5
+#endif
+// Which kernel (kw = 0: the one for few rows), queries per workgroup (128 or, with the waves in two key halves, 64)
+// and shares of the keys' length.
 void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& kw)
 {
     const int64_t heads = (int64_t)a->batch * a->heads;
-    kw = a->dtype == VK_DTYPE_F32 || heads * ((a->queries + 127) / 128) < 256 ? 2 : 1;
-    d.tiles = (a->queries + 128 / kw - 1) / (128 / kw);
-    const int64_t blocks = heads * d.tiles;
-    const int key_tiles = (a->keys + FWD_TILE - 1) / FWD_TILE;
-    int64_t splits = blocks >= 256 || blocks == 0 ? 1 : (512 + blocks - 1) / blocks;
-    splits = splits > (key_tiles + 1) / 2 ? (key_tiles + 1) / 2 : splits;
+    const int64_t rows = (int64_t)d.group * a->queries;
+    int64_t blocks, splits;
+    int key_tiles, least;                                       // tiles of the key axis, the fewest in a share
+    int row_tiles;
+    if (rows <= 64 || (double)heads * a->queries * a->keys <= NARROW_WORK) {
+        const int tk = a->dtype == VK_DTYPE_BF16 ? 128 : 64;
+        kw = 0;
+        d.tiles = (int)((rows + 15) / 16);
+        row_tiles = d.tiles;
+        blocks = (int64_t)a->batch * a->kv_heads * d.tiles;
+        key_tiles = (a->keys + tk - 1) / tk;
+        least = NWAVE;
+        splits = blocks == 0 ? 1 : (256 + blocks - 1) / blocks;
+    } else {
+        kw = a->dtype == VK_DTYPE_F32 || heads * ((a->queries + 127) / 128) < 256 ? 2 : 1;
+        d.tiles = (a->queries + 128 / kw - 1) / (128 / kw);
+        row_tiles = d.tiles * d.group;
+        blocks = heads * d.tiles;
+        key_tiles = (a->keys + FWD_TILE - 1) / FWD_TILE;
+        least = 2;
+        splits = blocks >= 256 || blocks == 0 ? 1 : (512 + blocks - 1) / blocks;
+    }
+    const int64_t most = (key_tiles + least - 1) / least;
+    if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     d.per_split = (int)((key_tiles + splits - 1) / splits);
+    if (kw == 0) d.per_split = (d.per_split + NWAVE - 1) / NWAVE * NWAVE;
     if (d.per_split < 1) d.per_split = 1;
     d.splits = (key_tiles + d.per_split - 1) / d.per_split;
     if (d.splits < 1) d.splits = 1;
-    vkba_place(d, (int64_t)d.tiles * d.splits * d.group);
+    vkba_place(d, (int64_t)row_tiles * d.splits);
 }
 
 }  // namespace
@@ -309,7 +348,8 @@ extern "C" int vk_bucket_attention(const vk_bucket_attention_args* a, void* stre
     d.part_ml = (float*)a->workspace;
     d.part_o = d.part_ml + (int64_t)d.splits * a->batch * a->heads * a->queries * 2;
     hipStream_t st = (hipStream_t)stream;
-    rc = a->dtype == VK_DTYPE_BF16 ? by_width<__bf16>(d, kw, st) : by_width<float>(d, kw, st);
+    if (kw == 0) rc = a->dtype == VK_DTYPE_BF16 ? narrow_by_width<__bf16>(d, st) : narrow_by_width<float>(d, st);
+    else rc = a->dtype == VK_DTYPE_BF16 ? by_width<__bf16>(d, kw, st) : by_width<float>(d, kw, st);
     if (rc != VK_OK || d.splits == 1) return rc;
     const int64_t n = (int64_t)a->batch * a->heads * a->head_dim * a->queries;
     dim3 grid((unsigned)((n + 255) / 256));

@@ -695,130 +695,108 @@ def rel_attention(qkv, emb_k, emb_v, mask, out, *, heads, window):
           "vk_rel_attention")
 
 
-def _on_device(device, launch):
-    """Run ``launch`` with ``device`` current (a launch goes to the current device's context)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return launch()
-    with torch.cuda.device(device):
-        return launch()
+# The calls below are made for sentences of a few dozen tokens too, where a kernel takes less time than the host
+# needs for a call: argument structs are built in one go, and nothing is formatted unless a LaunchTimer listens.
+
+def _on_device(index, launch, *args):
+    """Run ``launch`` with device ``index`` current (a launch goes to the current device's context)."""
+    if index == torch._C._cuda_getDevice():
+        return launch(*args)
+    with torch.cuda.device(index):
+        return launch(*args)
 
 
-def _bucket_args(q, k, v, out, lse, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
-    a = BucketAttentionArgs()
-    a.q, a.q_bstride, a.q_cstride = q.data_ptr(), q.stride(0), q.stride(1)
-    a.k, a.k_bstride, a.k_cstride = k.data_ptr(), k.stride(0), k.stride(1)
-    a.v, a.v_bstride, a.v_cstride = v.data_ptr(), v.stride(0), v.stride(1)
-    a.out, a.out_bstride, a.out_cstride = out.data_ptr(), out.stride(0), out.stride(1)
-    a.lse = lse.data_ptr()
-    if bias is not None:
-        a.bias, a.bucket_of = bias.data_ptr(), bucket_of.data_ptr()
-        a.has_bias, a.buckets, a.max_distance = 1, bias.shape[1], (bucket_of.shape[0] - 1) // 2
-    if key_lengths is not None:
-        a.key_lengths = key_lengths.data_ptr()
-    if query_lengths is not None:
-        a.query_lengths = query_lengths.data_ptr()
-    if query_start is not None:
-        a.query_start = query_start.data_ptr()
-    a.batch, a.heads, a.kv_heads, a.head_dim = q.shape[0], heads, kv_heads, q.shape[1] // heads
-    a.queries, a.keys = q.shape[2], k.shape[2]
-    a.causal, a.dtype, a.scale = int(causal), DTYPES[q.dtype], scale
-    return a
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
-def _bucket_run(name, a, device, family_flops, nbytes):
+def _view3(t):
+    """(pointer, batch stride, channel stride) of a [B, C, T] view; zeros for None."""
+    if t is None:
+        return None, 0, 0
+    st = t.stride()
+    return t.data_ptr(), st[0], st[1]
+
+
+def _run(entry, sizer, a, index, device, what, family, flops, nbytes, detail):
     """Size the workspace (stream-ordered, from torch's allocator: a graph keeps its own) and launch."""
-    L = lib()
+    ref = C.byref(a)
+    if sizer is not None:
+        need = sizer(ref)
+        if need:
+            check(min(need, 0), what)
+            ws = torch.empty(need, device=device, dtype=torch.uint8)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    sp = torch._C._cuda_getCurrentRawStream(index)
+    if LaunchTimer.active is None:
+        rc = entry(ref, sp)
+    else:
+        rc = _timed(family, flops(), nbytes(), device, lambda: entry(ref, sp), detail())
+    if rc:
+        check(rc, what)
 
-    def launch():
-        need = getattr(L, name + "_workspace_bytes")(C.byref(a))
-        check(min(need, 0), name)
-        ws = torch.empty(need, device=device, dtype=torch.uint8) if need else None
-        a.workspace, a.workspace_bytes = (ws.data_ptr() if need else None), need
-        sp = stream_ptr(device)
-        check(_timed(name[3:], family_flops, nbytes, device, lambda: getattr(L, name)(C.byref(a), sp),
-                     f"B{a.batch} H{a.heads}/{a.kv_heads} D{a.head_dim} Tq{a.queries} Tk{a.keys}"), name)
 
-    _on_device(device, launch)
+def _bucket(name, q, k, v, out, lse, grads, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths, query_start, causal,
+            scale):
+    assert q.is_cuda, "the HIP path needs device tensors"
+    dout, dq, dk, dv, dbias = grads
+    B, Cq, Tq = q.shape
+    Tk = k.shape[2]
+    a = BucketAttentionArgs(
+        *_view3(q), *_view3(k), *_view3(v), *_view3(out), lse.data_ptr(), *_view3(dout), *_view3(dq), *_view3(dk), *_view3(dv),
+        _ptr(dbias), _ptr(bias), _ptr(bucket_of), _ptr(key_lengths), _ptr(query_lengths), _ptr(query_start), None, 0,
+        B, heads, kv_heads, Cq // heads, Tq, Tk, bias is not None, bias.shape[1] if bias is not None else 0,
+        bucket_of.shape[0] // 2 if bias is not None else 0, bool(causal), DTYPES[q.dtype], scale)
+    L, device = lib(), q.device
+    backward = dout is not None
+    _on_device(device.index, _run, getattr(L, name), getattr(L, name + "_workspace_bytes"), a, device.index, device, name, name[3:],
+               lambda: (10.0 if backward else 4.0) * B * Cq * Tq * Tk,
+               lambda: (2 if backward else 1) * q.element_size() * (2 * q.numel() + k.numel() + v.numel()),
+               lambda: f"B{B} H{heads}/{kv_heads} D{Cq // heads} Tq{Tq} Tk{Tk}")
 
 
 def bucket_attention(q, k, v, out, lse, bias=None, bucket_of=None, *, heads, kv_heads, key_lengths=None,
                      query_lengths=None, query_start=None, causal=False, scale):
     """out, lse = attention of q over k, v with a bucketed relative position bias (``vk_bucket_attention``).
     Views [B, channels, T] with dense time; ``vits_amd.attention`` checks and allocates."""
-    assert q.is_cuda, "the HIP path needs device tensors"
-    a = _bucket_args(q, k, v, out, lse, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale)
-    _bucket_run("vk_bucket_attention", a, q.device, 4.0 * q.shape[0] * q.shape[1] * q.shape[2] * k.shape[2],
-                q.element_size() * (q.numel() + k.numel() + v.numel() + out.numel()))
+    _bucket("vk_bucket_attention", q, k, v, out, lse, (None,) * 5, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths,
+            query_start, causal, scale)
 
 
 def bucket_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, bias=None, bucket_of=None, dbias=None, *, heads, kv_heads,
                               key_lengths=None, query_lengths=None, query_start=None, causal=False, scale):
     """dq, dk, dv (and dbias) of ``bucket_attention`` (``vk_bucket_attention_backward``)."""
-    assert q.is_cuda, "the HIP path needs device tensors"
-    a = _bucket_args(q, k, v, out, lse, bias, bucket_of, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale)
-    a.dout, a.dout_bstride, a.dout_cstride = dout.data_ptr(), dout.stride(0), dout.stride(1)
-    a.dq, a.dq_bstride, a.dq_cstride = dq.data_ptr(), dq.stride(0), dq.stride(1)
-    a.dk, a.dk_bstride, a.dk_cstride = dk.data_ptr(), dk.stride(0), dk.stride(1)
-    a.dv, a.dv_bstride, a.dv_cstride = dv.data_ptr(), dv.stride(0), dv.stride(1)
-    if bias is not None:
-        a.dbias = dbias.data_ptr()
-    _bucket_run("vk_bucket_attention_backward", a, q.device, 10.0 * q.shape[0] * q.shape[1] * q.shape[2] * k.shape[2],
-                2 * q.element_size() * (q.numel() + k.numel() + v.numel() + out.numel()))
+    _bucket("vk_bucket_attention_backward", q, k, v, out, lse, (dout, dq, dk, dv, dbias), bias, bucket_of, heads, kv_heads,
+            key_lengths, query_lengths, query_start, causal, scale)
 
 
-def _block_norm_args(like, gate, scale, post, pre, norm, eps, lengths, **views):
-    a = BlockNormArgs()
-    for name, t in views.items():
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-            setattr(a, name + "_bstride", t.stride(0))
-            setattr(a, name + "_cstride", t.stride(1))
-    a.batch, a.channels, a.length = like.shape
-    if gate is not None:
-        a.gate, a.gate_bstride, a.gate_cstride = gate.data_ptr(), gate.stride(0), gate.stride(1)
-        a.gate_per_item = int(gate.shape[2] == 1 and like.shape[2] != 1)
-    for name, t in (("scale", scale), ("w_post", post and post[0]), ("b_post", post and post[1]), ("w_pre", pre and pre[0]),
-                    ("b_pre", pre and pre[1]), ("lengths", lengths)):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    a.norm, a.dtype, a.eps = norm, DTYPES[like.dtype], eps
-    return a
+def _norm(name, like, x, y, gate, scale, post, pre, h, n, lengths, grads, norm, eps):
+    assert like.is_cuda, "the HIP path needs device tensors"
+    dh, dn, dx, dy, dgate, dscale, dpost, dpre = grads
+    B, Cn, T = like.shape
+    none = (None, None)
+    a = BlockNormArgs(
+        *_view3(x), *_view3(y), *_view3(gate), _ptr(scale), *map(_ptr, post or none), *map(_ptr, pre or none), *_view3(h), *_view3(n),
+        _ptr(lengths), *_view3(dh), *_view3(dn), *_view3(dx), *_view3(dy), *_view3(dgate), _ptr(dscale), *map(_ptr, dpost or none),
+        *map(_ptr, dpre or none), None, 0, B, Cn, T, gate is not None and gate.shape[2] == 1 and T != 1, norm, DTYPES[like.dtype], eps)
+    L, device = lib(), like.device
+    _on_device(device.index, _run, getattr(L, name), L.vk_block_norm_backward_workspace_bytes if dx is not None else None, a,
+               device.index, device, name, name[3:], lambda: (20.0 if dx is None else 40.0) * like.numel(),
+               lambda: like.element_size() * sum(t.numel() for t in (x, y, gate, h, n, dh, dn, dx, dy, dgate) if t is not None),
+               lambda: f"B{B} C{Cn} T{T}")
 
 
 def block_norm(x, y, h, n, *, gate=None, scale=None, post=None, pre=None, norm=NORM_LAYER, eps=1e-5, lengths=None):
     """h = x + scale * gate * norm(y), n = norm(h) in one launch (``vk_block_norm``); y, h, n may be None.  ``post``, ``pre``:
     (weight, bias or None) or None.  ``vits_amd.block_norm`` checks and allocates."""
-    assert x.is_cuda, "the HIP path needs device tensors"
-    a = _block_norm_args(x, gate, scale, post, pre, norm, eps, lengths, x=x, y=y, h=h, n=n)
-    nbytes = x.element_size() * sum(t.numel() for t in (x, y, h, n, gate) if t is not None)
-    L = lib()
-    _on_device(x.device, lambda: check(
-        _timed("block_norm", 20.0 * x.numel(), nbytes, x.device, lambda: L.vk_block_norm(C.byref(a), stream_ptr(x.device)),
-               f"B{a.batch} C{a.channels} T{a.length}"), "vk_block_norm"))
+    _norm("vk_block_norm", x, x, y, gate, scale, post, pre, h, n, lengths, (None,) * 8, norm, eps)
 
 
 def block_norm_backward(dh, dn, h, y, dx, dy, *, gate=None, dgate=None, scale=None, dscale=None, post=None, dpost=None, pre=None,
                         dpre=None, norm=NORM_LAYER, eps=1e-5, lengths=None):
     """The gradients of ``block_norm`` (``vk_block_norm_backward``); ``dpost``, ``dpre`` like ``post``, ``pre``."""
-    assert dx.is_cuda, "the HIP path needs device tensors"
-    a = _block_norm_args(dx, gate, scale, post, pre, norm, eps, lengths, y=y, h=h, dh=dh, dn=dn, dx=dx, dy=dy, dgate=dgate)
-    for name, t in (("dscale", dscale), ("dw_post", dpost and dpost[0]), ("db_post", dpost and dpost[1]),
-                    ("dw_pre", dpre and dpre[0]), ("db_pre", dpre and dpre[1])):
-        if t is not None:
-            setattr(a, name, t.data_ptr())
-    nbytes = dx.element_size() * sum(t.numel() for t in (dh, dn, h, y, gate, dx, dy, dgate) if t is not None)
-    L = lib()
-
-    def launch():
-        need = L.vk_block_norm_backward_workspace_bytes(C.byref(a))
-        check(min(need, 0), "vk_block_norm_backward")
-        ws = torch.empty(need, device=dx.device, dtype=torch.uint8) if need else None
-        a.workspace, a.workspace_bytes = (ws.data_ptr() if need else None), need
-        check(_timed("block_norm_backward", 40.0 * dx.numel(), nbytes, dx.device,
-                     lambda: L.vk_block_norm_backward(C.byref(a), stream_ptr(dx.device)),
-                     f"B{a.batch} C{a.channels} T{a.length}"), "vk_block_norm_backward")
-
-    _on_device(dx.device, launch)
+    _norm("vk_block_norm_backward", dx, None, y, gate, scale, post, pre, h, None, lengths,
+          (dh, dn, dx, dy, dgate, dscale, dpost, dpre), norm, eps)
 
 
 EXPAND_MAX_TOKENS = 2048
