@@ -356,6 +356,19 @@ def test_views_of_larger_buffers(dtype):
 
 
 @gpu
+def test_saved_output_and_gradient_in_another_order():
+    """out and dout with the channels dense, as a transposed result of other code has them."""
+    b = RelativeBuckets(8, 20)
+    q, k, v, bias, dout = inputs(torch.float32, 2, 1, 1, 48, 37, 37, b)
+    out, lse = bucket_attention(q, k, v, bias, b, heads=1, return_lse=True)
+    turned = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)
+    assert turned(out).stride(2) != 1
+    for x, y in zip(bucket_attention_backward(dout, q, k, v, out, lse, bias, b, heads=1),
+                    bucket_attention_backward(turned(dout), q, k, v, turned(out), lse, bias, b, heads=1)):
+        assert torch.equal(x, y)
+
+
+@gpu
 def test_rows_around_the_outputs_stay_as_they_were():
     """Outputs written into views: nothing outside them is touched."""
     b = RelativeBuckets(8, 20)

@@ -132,8 +132,8 @@ def _forward(q, k, v, bias, table, heads, kv_heads, key_lengths, query_lengths, 
 
 
 def _backward(dout, q, k, v, out, lse, bias, table, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
-    if dout.stride(2) != 1 and dout.shape[2] > 1:           # gradients of sums come expanded
-        dout = dout.contiguous()
+    # gradients of sums come expanded, results of other code in another order
+    dout, out = (t if t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous() for t in (dout, out))
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     dbias = torch.empty_like(bias) if bias is not None else None
     native.bucket_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, bias, table, dbias, heads=heads, kv_heads=kv_heads,
@@ -197,12 +197,13 @@ def bucket_attention_backward(dout, q, k, v, out, lse, bias=None, buckets: Relat
                               kv_heads: int | None = None, key_lengths=None, query_lengths=None, query_start=None,
                               causal: bool = False, scale: float | None = None):
     """Gradients (dq, dk, dv, dbias) of ``bucket_attention`` for the gradient ``dout`` of its output, from what it took
-    and gave (``out``, ``lse``); dbias is None without a bias.  Every sum has a fixed order: the same inputs give the
+    and gave (``out``, ``lse``); dbias is None without a bias.  dout and out may have any strides (without a dense time
+    axis they are copied).  Every sum has a fixed order: the same inputs give the
     same bits.  Padding gets zero gradients."""
     kv_heads, scale, table = _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, query_start, scale)
-    _view3("out", out, q.dtype, q.device, q.shape)
-    if tuple(dout.shape) != tuple(q.shape) or dout.dtype != q.dtype or dout.device != q.device:
-        raise ValueError(f"dout must be {tuple(q.shape)} of {q.dtype} on {q.device}")
+    for name, t in (("dout", dout), ("out", out)):
+        if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{name} must be {tuple(q.shape)} of {q.dtype} on {q.device}")
     if tuple(lse.shape) != (q.shape[0], heads, q.shape[2]) or lse.dtype != torch.float32 or not lse.is_contiguous() \
             or lse.device != q.device:
         raise ValueError(f"lse must be a contiguous float32 [{q.shape[0]}, {heads}, {q.shape[2]}] on {q.device}")

@@ -89,8 +89,10 @@ def _backward(dh, dn, h, y, gate, scale, post, pre, norm, eps, lengths):
     dh, dn = _dense(dh), _dense(dn)
     like = dh if dh is not None else dn
     new = lambda t: t.new_empty(t.shape) if t is not None else None  # noqa: E731
-    par = lambda t: torch.empty_like(t) if t is not None else None  # noqa: E731
-    dx, dy, dgate, dscale = new(like), new(y), new(gate), par(scale)
+    dx, dy, dgate = new(like), new(y), new(gate)
+    row = iter(like.new_empty((5, like.shape[1]), dtype=torch.float32).unbind(0))     # the parameters' gradients: one allocation
+    par = lambda t: next(row) if t is not None else None  # noqa: E731
+    dscale = par(scale)
     dpost = (par(post[0]), par(post[1])) if post is not None else None
     dpre = (par(pre[0]), par(pre[1])) if pre is not None and dn is not None else None
     native.block_norm_backward(dh, dn, h, y, dx, dy, gate=gate, dgate=dgate, scale=scale, dscale=dscale, post=post, dpost=dpost,

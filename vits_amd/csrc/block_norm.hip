@@ -17,6 +17,7 @@
 #include "../../include/vits_amd.h"
 #include "api_internal.hpp"
 #include "chunk_load.hpp"
+#include "conv_mfma.hpp"      // vk_allow_lds
 
 namespace {
 
@@ -44,42 +45,51 @@ __device__ __forceinline__ void unpack(float (&v)[8], const u32x4& r)      // bf
         v[2 * e + 1] = __uint_as_float(r[e] & 0xffff0000u);
     }
 }
-// Columns t.. of a row of `length`; those at or behind `live` are written as 0.
-template <typename T, int E>
-__device__ __forceinline__ void store_cols(T* row, const float (&v)[E], int t, int length, int live)
+// Keeps the compiler from holding the unpacked values of a row between two uses: twice the registers in bf16.
+__device__ __forceinline__ void keep_packed(u32x4& r) { asm volatile("" : "+v"(r[0]), "+v"(r[1]), "+v"(r[2]), "+v"(r[3])); }
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)); }
+
+// Sum over the lanes of a wave that sit LT apart (LT <= 8): rotations within 16 lanes, then across.
+template <int LT>
+__device__ __forceinline__ float sum_apart(float v)
 {
-    T tmp[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) tmp[e] = t + e < live ? (T)v[e] : (T)0.0f;
-    if (t + E <= length) {
-        __builtin_memcpy(row + t, tmp, E * sizeof(T));
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) if (t + e < length) row[t + e] = tmp[e];
-    }
+    v += dpp<0x128>(v);                                     // rotate 16 lanes by 8
+    if constexpr (LT <= 4) v += dpp<0x124>(v);
+    if constexpr (LT <= 2) v += dpp<0x122>(v);
+    if constexpr (LT <= 1) v += dpp<0x121>(v);
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+// Sum over LT neighbouring lanes: within four, then a mirror of eight.
+template <int LT>
+__device__ __forceinline__ float sum_near(float v)
+{
+    if constexpr (LT >= 2) v += dpp<0xb1>(v);
+    if constexpr (LT >= 4) v += dpp<0x4e>(v);
+    if constexpr (LT >= 8) v += dpp<0x141>(v);
+    return v;
 }
 
-// Sum over the channel groups of a workgroup, for every column: lanes of one column group sit LT apart in a wave.
+// Sum over the channel groups of a workgroup, for every column.
 template <int LT, int E, int NW>
 __device__ __forceinline__ void column_sum(float (&v)[E], float* red)
 {
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, lt = lane % LT;
 #pragma unroll
-    for (int o = LT; o < 64; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] += __shfl_xor(v[e], o);
+    for (int e = 0; e < E; ++e) v[e] = sum_apart<LT>(v[e]);
     __syncthreads();                                        // the previous sum has been read
     if (lane < LT)
 #pragma unroll
         for (int e = 0; e < E; ++e) red[(wave * LT + lt) * E + e] = v[e];
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        float s = 0.0f;
+    for (int e = 0; e < E; ++e) v[e] = 0.0f;
+#pragma unroll 2                                            // all NW * E reads at once would take as many registers
+    for (int w = 0; w < NW; ++w)
 #pragma unroll
-        for (int w = 0; w < NW; ++w) s += red[(w * LT + lt) * E + e];
-        v[e] = s;
-    }
+        for (int e = 0; e < E; ++e) v[e] += red[(w * LT + lt) * E + e];
 }
 
 // Per column: mean (0 for rms) and 1 / sqrt(mean square about it + eps) of rows value(r, v), r < rows.  Two sweeps
@@ -120,37 +130,120 @@ __device__ __forceinline__ void column_stats(F value, int rows, int channels, fl
 }
 
 // Where a thread works: channels cg, cg + CG, .. (`rows` of them), columns t .. t + E - 1 of item b, of which those
-// before `live` count.  LT lanes along time, the other lanes and the waves along the channels.
+// before `live` count.  LT lanes along time, the other lanes and the waves along the channels.  An address is the
+// item's base (uniform) and a 32-bit offset, which the rows of a thread share but for a uniform part.
 template <typename T, int LT, int NW>
 struct Spot {
     static constexpr int E = Pack<T>::E, CG = 64 / LT * NW;
-    int cg, rows, b, t, live, lt, channels;
+    int cg, rows, b, t, live, length, lt, channels, id;
+    bool any, inside, tiny;         // a window at all; all of it live; rows shorter than a chunk
+    int at, moved;                  // where this thread's chunks are read, and how far that is before t
+    u32x4 keep;                     // the live columns as bits, where not all are
     __device__ __forceinline__ Spot(const NDev& p)
     {
         const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
         lt = lane % LT;
         cg = wave * (64 / LT) + lane / LT;
-        b = (int)blockIdx.x / p.windows;
-        t = ((int)blockIdx.x - b * p.windows) * LT * E + lt * E;
+        // neighbouring windows share cache lines at their borders (and, narrower than a line, everywhere): they go to
+        // one XCD, which takes every eighth workgroup
+        const int n = p.a.batch * p.windows, per = (n + 7) >> 3;
+        id = ((int)blockIdx.x & 7) * per + ((int)blockIdx.x >> 3);
+        any = ((int)blockIdx.x >> 3) < per && id < n;
+        b = id / p.windows;
+        const int t0 = (id - b * p.windows) * LT * E;
+        t = t0 + lt * E;
         channels = p.a.channels;
-        live = p.a.length;
-        if (p.a.lengths) { const int64_t n = p.a.lengths[b]; live = (int)(n < 0 ? 0 : n > p.a.length ? p.a.length : n); }
-        rows = cg < p.a.channels ? (p.a.channels - cg + CG - 1) / CG : 0;
+        live = length = p.a.length;
+        if (p.a.lengths && any) { const int64_t m = p.a.lengths[b]; live = __builtin_amdgcn_readfirstlane((int)(m < 0 ? 0 : m > length ? length : m)); }
+        rows = cg < channels ? (channels - cg + CG - 1) / CG : 0;
+        inside = t0 + LT * E <= live;
+        tiny = length < E;
+        at = min(t, max(length - E, 0));
+        moved = min(t - at, E);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (E == 4) keep[j] = t + j < live ? 0xffffffffu : 0u;
+            else keep[j] = (t + 2 * j < live ? 0xffffu : 0u) | (t + 2 * j + 1 < live ? 0xffff0000u : 0u);
+        }
     }
-    __device__ __forceinline__ int channel(int r) const { return cg + r * CG; }
+    // Threads without a channel take their first (or channel 0) again and store nothing: no branches around the loads.
+    __device__ __forceinline__ int channel(int r) const { return r < rows ? cg + r * CG : rows ? cg : 0; }
+    // Byte offset of row r at column `col`.  Computed where it is used: held for all rows and tensors, the offsets
+    // would take more registers than the data.
+    __device__ __forceinline__ unsigned offset(int64_t cstride, int col, int r) const
+    {
+        unsigned o = ((unsigned)(rows ? cg : 0) * (unsigned)cstride + (unsigned)col) * (unsigned)sizeof(T);
+        asm volatile("" : "+v"(o));
+        return r < rows ? o + (unsigned)r * (unsigned)CG * (unsigned)cstride * (unsigned)sizeof(T) : o;
+    }
+    __device__ __forceinline__ u32x4 load_row(const void* base, int64_t bstride, int64_t cstride, int r) const
+    {
+        const char* row = (const char*)((const T*)base + (int64_t)b * bstride);
+        const unsigned off = offset(cstride, at, r);
+        u32x4 c;
+        if (tiny) {
+            unsigned long long v[2] = {0, 0};
+#pragma unroll 1
+            for (int e = 0; e < length; ++e) {
+                const T x = *(const T*)(row + off + e * sizeof(T));
+                unsigned bits = 0;
+                __builtin_memcpy(&bits, &x, sizeof(T));
+                const int pos = e * 8 * (int)sizeof(T);
+                v[0] |= pos < 64 ? (unsigned long long)bits << pos : 0;
+                v[1] |= pos >= 64 ? (unsigned long long)bits << (pos - 64) : 0;
+            }
+            c = u32x4{(unsigned)v[0], (unsigned)(v[0] >> 32), (unsigned)v[1], (unsigned)(v[1] >> 32)};
+        } else {
+            __builtin_memcpy(&c, row + off, 16);
+        }
+        if (!inside) c = chunk_shift<E>(c, moved) & keep;
+        return c;
+    }
     template <int R>
     __device__ __forceinline__ void load(u32x4 (&v)[R], const void* base, int64_t bstride, int64_t cstride) const
     {
-        // threads without a channel read the last one again: the loads stay free of branches
-        const T* p = (const T*)base + (int64_t)b * bstride;
 #pragma unroll
-        for (int r = 0; r < R; ++r) v[r] = load_chunk<T>(p + (int64_t)min(channel(r), channels - 1) * cstride, t, live);
+        for (int r = 0; r < R; ++r) v[r] = load_row(base, bstride, cstride, r);
     }
-    __device__ __forceinline__ T* row(void* base, int64_t bstride, int64_t cstride, int r) const
+    __device__ __forceinline__ void store_row(void* base, int64_t bstride, int64_t cstride, int r, const float (&v)[E]) const
     {
-        return (T*)base + (int64_t)b * bstride + (int64_t)channel(r) * cstride;
+        if (r >= rows) return;
+        char* row = (char*)((T*)base + (int64_t)b * bstride);
+        const unsigned off = offset(cstride, t, r);
+        T tmp[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) tmp[e] = (T)v[e];
+        u32x4 c;
+        __builtin_memcpy(&c, tmp, 16);
+        if (!inside) c &= keep;
+        if (inside || t + E <= length) {
+            __builtin_memcpy(row + off, &c, 16);
+        } else {
+            unsigned long long q[2] = {c[0] | (unsigned long long)c[1] << 32, c[2] | (unsigned long long)c[3] << 32};
+#pragma unroll 1
+            for (int e = 0; e < length - t; ++e) {
+                const int pos = e * 8 * (int)sizeof(T);
+                const unsigned bits = (unsigned)(pos < 64 ? q[0] >> pos : q[1] >> (pos - 64));
+                __builtin_memcpy(row + off + e * sizeof(T), &bits, sizeof(T));
+            }
+        }
     }
 };
+
+// The per-channel numbers of a pass in LDS: ones and zeros where something is not given.
+enum { P_SCALE, P_GATE, P_WPOST, P_BPOST, P_WPRE, P_BPRE, P_COUNT };
+template <typename T>
+__device__ __forceinline__ void stage_params(float* par, const vk_block_norm_args& a, int b)
+{
+    const bool item = a.gate && a.gate_per_item;
+    const float* src[P_COUNT] = {a.scale, nullptr, a.w_post, a.b_post, a.w_pre, a.b_pre};
+    for (int c = (int)threadIdx.x; c < a.channels; c += (int)blockDim.x) {
+#pragma unroll
+        for (int i = 0; i < P_COUNT; ++i)
+            if (i != P_GATE) par[i * a.channels + c] = src[i] ? src[i][c] : (i == P_BPOST || i == P_BPRE) ? 0.0f : 1.0f;
+        par[P_GATE * a.channels + c] = item ? (float)((const T*)a.gate)[(int64_t)b * a.gate_bstride + (int64_t)c * a.gate_cstride] : 1.0f;
+    }
+}
 
 template <typename T, int LT, int NW, int R>
 __global__ __launch_bounds__(64 * NW)
@@ -158,92 +251,86 @@ void block_norm_kernel(NDev p)
 {
     using S = Spot<T, LT, NW>;
     constexpr int E = S::E;
-    __shared__ float red[NW * LT * E];
+    extern __shared__ __align__(16) float lds[];
+    float* red = lds;
+    float* par = lds + NW * LT * E;
     const vk_block_norm_args& a = p.a;
     const S at(p);
-    const bool layer = a.norm == VK_NORM_LAYER;
-    u32x4 xr[R], yr[R], gr[R];
-    at.load(xr, a.x, a.x_bstride, a.x_cstride);
+    if (!at.any) return;
+    const int C = a.channels;
+    const bool layer = a.norm == VK_NORM_LAYER, full_gate = a.gate && !a.gate_per_item;
+    u32x4 xr[R], yr[R];
     if (a.y) at.load(yr, a.y, a.y_bstride, a.y_cstride);
-    if (a.gate && !a.gate_per_item) at.load(gr, a.gate, a.gate_bstride, a.gate_cstride);
+    at.load(xr, a.x, a.x_bstride, a.x_cstride);
+    stage_params<T>(par, a, at.b);
+    __syncthreads();
     float h[R][E];
-#pragma unroll
-    for (int r = 0; r < R; ++r) unpack(h[r], xr[r]);
     if (a.y) {
         float mean[E], rstd[E];
-        if (a.w_post) column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) { unpack(v, yr[r]); }, at.rows, a.channels, a.eps, layer, red, mean, rstd);
+        if (a.w_post) column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) { unpack(v, yr[r]); keep_packed(yr[r]); }, at.rows, C, a.eps, layer, red, mean, rstd);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (r >= at.rows) continue;
-            const int c = at.channel(r);
-            const float s = a.scale ? a.scale[c] : 1.0f;
+            const float* q = par + at.channel(r);
+            const float s = q[P_SCALE * C] * q[P_GATE * C], w = q[P_WPOST * C], bias = q[P_BPOST * C];
             float g[E], z[E];
-            if (a.gate && !a.gate_per_item) {
-                unpack(g, gr[r]);
-#pragma unroll
-                for (int e = 0; e < E; ++e) g[e] *= s;
-            } else {
-                const float q = a.gate ? s * (float)((const T*)a.gate)[(int64_t)at.b * a.gate_bstride + (int64_t)c * a.gate_cstride] : s;
-#pragma unroll
-                for (int e = 0; e < E; ++e) g[e] = q;
-            }
+            if (full_gate) unpack(g, at.load_row(a.gate, a.gate_bstride, a.gate_cstride, r));
             unpack(z, yr[r]);
-            if (a.w_post) {
-                const float w = a.w_post[c], bias = a.b_post ? a.b_post[c] : 0.0f;
+            unpack(h[r], xr[r]);
 #pragma unroll
-                for (int e = 0; e < E; ++e) z[e] = fmaf((z[e] - mean[e]) * rstd[e], w, bias);
+            for (int e = 0; e < E; ++e) {
+                if (a.w_post) z[e] = fmaf((z[e] - mean[e]) * rstd[e], w, bias);
+                h[r][e] = fmaf(full_gate ? g[e] * s : s, z[e], h[r][e]);
             }
-#pragma unroll
-            for (int e = 0; e < E; ++e) h[r][e] = fmaf(g[e], z[e], h[r][e]);
-            if (a.h) store_cols<T, E>(at.row(a.h, a.h_bstride, a.h_cstride, r), h[r], at.t, a.length, at.live);
         }
-    } else if (a.h) {
+    } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (r < at.rows) store_cols<T, E>(at.row(a.h, a.h_bstride, a.h_cstride, r), h[r], at.t, a.length, at.live);
+        for (int r = 0; r < R; ++r) unpack(h[r], xr[r]);
     }
-    if (a.n) {
-        float mean[E], rstd[E];
-        column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) {
+    if (a.h)
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = h[r][e]; }, at.rows, a.channels, a.eps, layer, red, mean, rstd);
+        for (int r = 0; r < R; ++r) at.store_row(a.h, a.h_bstride, a.h_cstride, r, h[r]);
+    if (!a.n) return;
+    float mean[E], rstd[E];
+    column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            if (r >= at.rows) continue;
-            const int c = at.channel(r);
-            const float w = a.w_pre[c], bias = a.b_pre ? a.b_pre[c] : 0.0f;
-            float o[E];
+        for (int e = 0; e < E; ++e) v[e] = h[r][e]; }, at.rows, C, a.eps, layer, red, mean, rstd);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf((h[r][e] - mean[e]) * rstd[e], w, bias);
-            store_cols<T, E>(at.row(a.n, a.n_bstride, a.n_cstride, r), o, at.t, a.length, at.live);
-        }
+    for (int r = 0; r < R; ++r) {
+        const float* q = par + at.channel(r);
+        const float w = q[P_WPRE * C], bias = q[P_BPRE * C];
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf((h[r][e] - mean[e]) * rstd[e], w, bias);
+        at.store_row(a.n, a.n_bstride, a.n_cstride, r, o);
     }
 }
 
 // Gradient through a norm: g -> (g - mean(g) - vhat * mean(g * vhat)) * rstd (layer; without mean(g) for rms).
 //
 // The gradient of h stays in registers in fp32 from the norm before the next block to the norm after this one.
-// Parameter gradients are sums over the columns of a row: over the lanes of a column group (shuffles), then one
-// number per row and workgroup goes to memory, and a second kernel adds the workgroups in a fixed order.
+// Parameter gradients are sums over the columns of a row: over the lanes of a column group, then one number per
+// row and workgroup goes to memory, and a second kernel adds the workgroups in a fixed order.
 template <typename T, int LT, int NW, int R>
 __global__ __launch_bounds__(64 * NW)
 void block_norm_backward_kernel(NDev p)
 {
     using S = Spot<T, LT, NW>;
     constexpr int E = S::E;
-    __shared__ float red[NW * LT * E];
+    extern __shared__ __align__(16) float lds[];
+    float* red = lds;
+    float* par = lds + NW * LT * E;
     const vk_block_norm_args& a = p.a;
     const S at(p);
-    const bool layer = a.norm == VK_NORM_LAYER;
-    const float inv = 1.0f / (float)a.channels;
-    float* part = p.part + (int64_t)blockIdx.x * 5 * a.channels;
+    if (!at.any) return;
+    const int C = a.channels;
+    const bool layer = a.norm == VK_NORM_LAYER, full_gate = a.gate && !a.gate_per_item, item_gate = a.dgate && a.gate_per_item;
+    const float inv = 1.0f / (float)C;
+    float* part = p.part + (int64_t)at.id * 5 * C;
     auto over_columns = [&](const float (&x)[E]) {
         float s = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) s += x[e];
-#pragma unroll
-        for (int o = 1; o < LT; o <<= 1) s += __shfl_xor(s, o);
-        return s;
+        return sum_near<LT>(s);
     };
 
     float g[R][E];              // gradient of h, then of z
@@ -251,27 +338,29 @@ void block_norm_backward_kernel(NDev p)
         u32x4 hr[R], dr[R];
         at.load(hr, a.h, a.h_bstride, a.h_cstride);
         at.load(dr, a.dn, a.dn_bstride, a.dn_cstride);
+        stage_params<T>(par, a, at.b);
+        __syncthreads();
         float mean[E], rstd[E], m1[E], m2[E];
-        column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) { unpack(v, hr[r]); }, at.rows, a.channels, a.eps, layer, red, mean, rstd);
+        column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) { unpack(v, hr[r]); keep_packed(hr[r]); }, at.rows, C, a.eps, layer, red, mean, rstd);
 #pragma unroll
         for (int e = 0; e < E; ++e) m1[e] = m2[e] = 0.0f;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (r >= at.rows) continue;
             const int c = at.channel(r);
-            const float w = a.w_pre[c];
+            const float w = r < at.rows ? par[P_WPRE * C + c] : 0.0f;       // a repeated channel counts once
             float v[E], d[E], dw[E];
             unpack(v, hr[r]);
             unpack(d, dr[r]);
+            keep_packed(hr[r]);
+            keep_packed(dr[r]);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float vh = (v[e] - mean[e]) * rstd[e];
-                dw[e] = d[e] * vh;
+                dw[e] = d[e] * ((v[e] - mean[e]) * rstd[e]);
                 m1[e] = fmaf(d[e], w, m1[e]);
                 m2[e] = fmaf(dw[e], w, m2[e]);
             }
             const float sw = over_columns(dw), sb = over_columns(d);
-            if (at.lt == 0) { part[c] = sw; part[a.channels + c] = sb; }
+            if (at.lt == 0 && r < at.rows) { part[c] = sw; part[C + c] = sb; }
         }
         if (layer) column_sum<LT, E, NW>(m1, red);
         column_sum<LT, E, NW>(m2, red);
@@ -279,7 +368,7 @@ void block_norm_backward_kernel(NDev p)
         for (int e = 0; e < E; ++e) { m1[e] = layer ? m1[e] * inv : 0.0f; m2[e] *= inv; }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const float w = r < at.rows ? a.w_pre[at.channel(r)] : 0.0f;
+            const float w = par[P_WPRE * C + at.channel(r)];
             float v[E], d[E];
             unpack(v, hr[r]);
             unpack(d, dr[r]);
@@ -287,65 +376,61 @@ void block_norm_backward_kernel(NDev p)
             for (int e = 0; e < E; ++e) g[r][e] = (fmaf(d[e], w, -m1[e]) - (v[e] - mean[e]) * rstd[e] * m2[e]) * rstd[e];
         }
     } else {
+        stage_params<T>(par, a, at.b);
+        __syncthreads();
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int e = 0; e < E; ++e) g[r][e] = 0.0f;
     }
-    u32x4 yr[R];
-    if (a.y) at.load(yr, a.y, a.y_bstride, a.y_cstride);
+    if (a.dh)
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (r >= at.rows) continue;
-        if (a.dh) {
+        for (int r = 0; r < R; ++r) {
             float d[E];
-            unpack(d, load_chunk<T>((const T*)a.dh + (int64_t)at.b * a.dh_bstride + (int64_t)at.channel(r) * a.dh_cstride, at.t, at.live));
+            unpack(d, at.load_row(a.dh, a.dh_bstride, a.dh_cstride, r));
 #pragma unroll
             for (int e = 0; e < E; ++e) g[r][e] += d[e];
         }
-        store_cols<T, E>(at.row(a.dx, a.dx_bstride, a.dx_cstride, r), g[r], at.t, a.length, at.live);
-    }
+    u32x4 yr[R];
+    if (a.y) at.load(yr, a.y, a.y_bstride, a.y_cstride);
+#pragma unroll
+    for (int r = 0; r < R; ++r) at.store_row(a.dx, a.dx_bstride, a.dx_cstride, r, g[r]);
     if (!a.y) return;
 
     float mean[E], rstd[E], m1[E], m2[E];
-    if (a.w_post) column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) { unpack(v, yr[r]); }, at.rows, a.channels, a.eps, layer, red, mean, rstd);
+    if (a.w_post) column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) { unpack(v, yr[r]); keep_packed(yr[r]); }, at.rows, C, a.eps, layer, red, mean, rstd);
 #pragma unroll
     for (int e = 0; e < E; ++e) m1[e] = m2[e] = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (r >= at.rows) continue;
         const int c = at.channel(r);
-        const float s = a.scale ? a.scale[c] : 1.0f;
-        const float w = a.w_post ? a.w_post[c] : 1.0f, bias = a.b_post ? a.b_post[c] : 0.0f;
+        const float* q = par + c;
+        const float s = q[P_SCALE * C], w = q[P_WPOST * C], bias = q[P_BPOST * C], gi = q[P_GATE * C];
         float gate[E], dg[E], ds[E], dw[E], v[E];
-        if (a.gate && !a.gate_per_item) {
-            unpack(gate, load_chunk<T>((const T*)a.gate + (int64_t)at.b * a.gate_bstride + (int64_t)c * a.gate_cstride, at.t, at.live));
-        } else {
-            const float q = a.gate ? (float)((const T*)a.gate)[(int64_t)at.b * a.gate_bstride + (int64_t)c * a.gate_cstride] : 1.0f;
-#pragma unroll
-            for (int e = 0; e < E; ++e) gate[e] = q;
-        }
+        if (full_gate) unpack(gate, at.load_row(a.gate, a.gate_bstride, a.gate_cstride, r));
         unpack(v, yr[r]);
+        keep_packed(yr[r]);
+        const float wm = r < at.rows ? w : 0.0f;        // a repeated channel counts once
 #pragma unroll
         for (int e = 0; e < E; ++e) {
+            const float ge = full_gate ? gate[e] : gi;
             if (a.w_post) v[e] = (v[e] - mean[e]) * rstd[e];
             const float z = a.w_post ? fmaf(v[e], w, bias) : v[e];
             dg[e] = g[r][e] * s * z;                    // gradient of the gate
-            ds[e] = g[r][e] * gate[e] * z;              // of the scale
-            g[r][e] *= s * gate[e];                     // of z
+            ds[e] = g[r][e] * ge * z;                   // of the scale
+            g[r][e] *= s * ge;                          // of z
             dw[e] = g[r][e] * v[e];                     // of the weight
-            m1[e] = fmaf(g[r][e], w, m1[e]);
-            m2[e] = fmaf(dw[e], w, m2[e]);
+            m1[e] = fmaf(g[r][e], wm, m1[e]);
+            m2[e] = fmaf(dw[e], wm, m2[e]);
         }
-        if (a.dgate && !a.gate_per_item)
-            store_cols<T, E>(at.row(a.dgate, a.dgate_bstride, a.dgate_cstride, r), dg, at.t, a.length, at.live);
-        const float sg = a.dgate && a.gate_per_item ? over_columns(dg) : 0.0f;
+        if (a.dgate && full_gate) at.store_row(a.dgate, a.dgate_bstride, a.dgate_cstride, r, dg);
+        const float sg = item_gate ? over_columns(dg) : 0.0f;
         const float ss = over_columns(ds), sw = over_columns(dw), sb = over_columns(g[r]);
-        if (at.lt == 0) {
-            part[2 * a.channels + c] = ss;
-            part[3 * a.channels + c] = sw;
-            part[4 * a.channels + c] = sb;
-            if (a.dgate && a.gate_per_item) p.part_gate[(int64_t)blockIdx.x * a.channels + c] = sg;
+        if (at.lt == 0 && r < at.rows) {
+            part[2 * C + c] = ss;
+            part[3 * C + c] = sw;
+            part[4 * C + c] = sb;
+            if (item_gate) p.part_gate[(int64_t)at.id * C + c] = sg;
         }
     }
     if (a.w_post) {
@@ -356,20 +441,19 @@ void block_norm_backward_kernel(NDev p)
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        if (r >= at.rows) continue;
         if (a.w_post) {
-            const float w = a.w_post[at.channel(r)];
+            const float w = par[P_WPOST * C + at.channel(r)];
             float v[E];
             unpack(v, yr[r]);
 #pragma unroll
             for (int e = 0; e < E; ++e) g[r][e] = (fmaf(g[r][e], w, -m1[e]) - (v[e] - mean[e]) * rstd[e] * m2[e]) * rstd[e];
         }
-        store_cols<T, E>(at.row(a.dy, a.dy_bstride, a.dy_cstride, r), g[r], at.t, a.length, at.live);
+        at.store_row(a.dy, a.dy_bstride, a.dy_cstride, r, g[r]);
     }
 }
 
 // Sums over the workgroups: blockIdx.y 0..4 a parameter's gradient, 5.. the gate of item blockIdx.y - 5.
-constexpr int SUM_C = 32, SUM_P = 8;
+constexpr int SUM_C = 32, SUM_P = 32;
 template <typename T>
 __global__ __launch_bounds__(SUM_C * SUM_P)
 void block_norm_sums_kernel(NDev p)
@@ -384,6 +468,7 @@ void block_norm_sums_kernel(NDev p)
     const float* src = which < 5 ? p.part + (int64_t)which * a.channels : p.part_gate + (int64_t)(which - 5) * p.windows * a.channels;
     float s = 0.0f;
     if (c < a.channels)
+#pragma unroll 4
         for (int i = q; i < n; i += SUM_P) s += src[i * stride + c];
     acc[q][threadIdx.x % SUM_C] = s;
     __syncthreads();
@@ -398,6 +483,12 @@ int fail(int code, const char* what, const char* msg)
     char buf[256];
     snprintf(buf, sizeof(buf), "%s: %s", what, msg);
     return vk_fail(code, buf);
+}
+
+// Rows of one item are addressed with 32-bit offsets.
+bool item_fits(const void* p, int64_t cstride, const vk_block_norm_args* a)
+{
+    return !p || ((int64_t)(a->channels - 1) * (cstride < 0 ? -cstride : cstride) + a->length) * 4 < (int64_t)1 << 32;
 }
 
 bool rows_apart(int64_t bstride, int64_t cstride, const vk_block_norm_args* a)
@@ -418,6 +509,11 @@ int check(const vk_block_norm_args* a, const char* what, bool backward)
     const bool some = a->batch > 0 && a->length > 0;
     if (some && !a->y && (a->gate || a->scale || a->w_post)) return fail(VK_E_ARG, what, "gate, scale and the norm after the block need y");
     if ((!a->w_post && a->b_post) || (!a->w_pre && a->b_pre)) return fail(VK_E_ARG, what, "a norm's bias needs its weight");
+    if (!item_fits(a->x, a->x_cstride, a) || !item_fits(a->y, a->y_cstride, a) || !item_fits(a->h, a->h_cstride, a)
+        || !item_fits(a->n, a->n_cstride, a) || !item_fits(a->dh, a->dh_cstride, a) || !item_fits(a->dn, a->dn_cstride, a)
+        || !item_fits(a->dx, a->dx_cstride, a) || !item_fits(a->dy, a->dy_cstride, a)
+        || (!a->gate_per_item && (!item_fits(a->gate, a->gate_cstride, a) || !item_fits(a->dgate, a->dgate_cstride, a))))
+        return fail(VK_E_UNSUPPORTED, what, "an item's view spans 2^30 elements or more");
     if (!backward) {
         if (some && (!a->x || (!a->h && !a->n))) return fail(VK_E_ARG, what, "null x, or nothing to write");
         if (some && a->n && !a->w_pre) return fail(VK_E_ARG, what, "n needs w_pre");
@@ -443,10 +539,10 @@ int check(const vk_block_norm_args* a, const char* what, bool backward)
 struct Plan { int lt, nw, r; };
 Plan plan_of(const vk_block_norm_args* a)
 {
-    static constexpr int kShapes[4][2] = {{4, 4}, {4, 8}, {8, 8}, {8, 16}};
-    const int e = a->dtype == VK_DTYPE_BF16 ? 8 : 4, top = 64 / e;      // at most 64 values of a tensor per thread
-    Plan pl{8, 8, top};
-    while (pl.lt > 1 && (64 / pl.lt) * 8 * top < a->channels) pl.lt >>= 1;
+    static constexpr int kShapes[3][2] = {{4, 4}, {4, 8}, {8, 8}};
+    const int e = a->dtype == VK_DTYPE_BF16 ? 8 : 4;
+    Plan pl{8, 8, 8};
+    while (pl.lt > 1 && (64 / pl.lt) * kShapes[2][0] * kShapes[2][1] < a->channels) pl.lt >>= 1;
     // fewer than 256 workgroups: narrower windows spread over more CUs
     while (pl.lt > 1 && (int64_t)a->batch * ((a->length + pl.lt * e - 1) / (pl.lt * e)) < 256) pl.lt >>= 1;
     for (const auto& s : kShapes)
@@ -454,15 +550,25 @@ Plan plan_of(const vk_block_norm_args* a)
     return pl;
 }
 
+template <auto KERNEL>
+int launch_kernel(const NDev& d, int64_t blocks, int threads, size_t lds, hipStream_t st, const char* what)
+{
+    static std::atomic<unsigned long long> raised{0};
+    hipError_t e = vk_allow_lds(KERNEL, lds, raised);
+    if (e != hipSuccess) return fail(VK_E_LAUNCH, what, hipGetErrorString(e));
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3(threads), lds, st, d);
+    e = hipGetLastError();
+    return e == hipSuccess ? VK_OK : fail(VK_E_LAUNCH, what, hipGetErrorString(e));
+}
+
 template <typename T, int LT, int NW, int R>
 int launch(const NDev& d, bool backward, hipStream_t st, const char* what)
 {
-    const int64_t blocks = (int64_t)d.a.batch * d.windows;
+    const int64_t blocks = ((int64_t)d.a.batch * d.windows + 7) / 8 * 8;       // see Spot
     if (blocks > 0x7fffffff) return fail(VK_E_UNSUPPORTED, what, "too many workgroups");
-    if (backward) hipLaunchKernelGGL((block_norm_backward_kernel<T, LT, NW, R>), dim3((unsigned)blocks), dim3(64 * NW), 0, st, d);
-    else hipLaunchKernelGGL((block_norm_kernel<T, LT, NW, R>), dim3((unsigned)blocks), dim3(64 * NW), 0, st, d);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? VK_OK : fail(VK_E_LAUNCH, what, hipGetErrorString(e));
+    const size_t lds = (NW * LT * Pack<T>::E + P_COUNT * (size_t)d.a.channels) * 4;
+    return backward ? launch_kernel<block_norm_backward_kernel<T, LT, NW, R>>(d, blocks, 64 * NW, lds, st, what)
+                    : launch_kernel<block_norm_kernel<T, LT, NW, R>>(d, blocks, 64 * NW, lds, st, what);
 }
 template <typename T, int NW, int R>
 int by_window(const NDev& d, int lt, bool backward, hipStream_t st, const char* what)
@@ -477,10 +583,8 @@ int by_window(const NDev& d, int lt, bool backward, hipStream_t st, const char* 
 template <typename T>
 int by_shape(const NDev& d, const Plan& pl, bool backward, hipStream_t st, const char* what)
 {
-    if (pl.nw == 4) return pl.r == 4 ? by_window<T, 4, 4>(d, pl.lt, backward, st, what) : by_window<T, 4, 8>(d, pl.lt, backward, st, what);
-    if constexpr (Pack<T>::E == 4)
-        if (pl.r == 16) return by_window<T, 8, 16>(d, pl.lt, backward, st, what);
-    return by_window<T, 8, 8>(d, pl.lt, backward, st, what);
+    if (pl.nw == 4 && pl.r == 4) return by_window<T, 4, 4>(d, pl.lt, backward, st, what);
+    return pl.nw == 4 ? by_window<T, 4, 8>(d, pl.lt, backward, st, what) : by_window<T, 8, 8>(d, pl.lt, backward, st, what);
 }
 
 int windows_of(const vk_block_norm_args* a, const Plan& pl)
