@@ -214,7 +214,7 @@ void bucket_attention_kernel(Dev p)
 }
 
 // Joins the shares of the keys: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, m = max m_s.
-// One thread per query and channel block of a head.
+// One thread per query and channel of a head; the shares' numbers are requested eight at a time.
 template <typename T>
 __global__ __launch_bounds__(256)
 void bucket_attention_join_kernel(Dev p)
@@ -225,17 +225,30 @@ void bucket_attention_join_kernel(Dev p)
     if (e >= rows * p.head_dim) return;
     const int64_t bh = e / per_head, rem = e - bh * per_head;
     const int d = (int)(rem / p.queries), qi = (int)(rem - (int64_t)d * p.queries);
-    const int64_t row = bh * p.queries + qi;
-    float m = -__builtin_inff();
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[((int64_t)s * rows + row) * 2]);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-    float o = 0.0f, total = 0.0f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float l = p.part_ml[((int64_t)s * rows + row) * 2 + 1];
-        const float w = exp2_hw(p.part_ml[((int64_t)s * rows + row) * 2] - base);
-        if (l != 0.0f) {
-            total = fmaf(w, l, total);
-            o = fmaf(w, p.part_o[((int64_t)s * p.batch * p.heads + bh) * per_head + rem], o);
+    const int64_t row = bh * p.queries + qi, o_step = (int64_t)p.batch * p.heads * per_head;
+    float m = -__builtin_inff(), o = 0.0f, total = 0.0f;
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {
+        float ms[8], ls[8], os[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t s = min(s0 + i, p.splits - 1);
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * rows + row) * 2);
+            ms[i] = s0 + i < p.splits ? ml.x : -__builtin_inff();
+            ls[i] = s0 + i < p.splits ? ml.y : 0.0f;
+            os[i] = p.part_o[s * o_step + bh * per_head + rem];
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, ms[i]);
+        const float base = top == -__builtin_inff() ? 0.0f : top, keep = exp2_hw(m - base);
+        o *= keep;
+        total *= keep;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float w = exp2_hw(ms[i] - base);
+            total = fmaf(w, ls[i], total);
+            o = ls[i] != 0.0f ? fmaf(w, os[i], o) : o;     // a share without keys left its sums unwritten
         }
     }
     const int b = (int)(bh / p.heads), head = (int)(bh - (int64_t)b * p.heads);
@@ -292,7 +305,8 @@ void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& kw)
     int64_t blocks, splits;
     int key_tiles, least;                                       // tiles of the key axis, the fewest in a share
     int row_tiles;
-    if (rows <= 64 || (double)heads * a->queries * a->keys <= NARROW_WORK) {
+    const int chunk = a->dtype == VK_DTYPE_BF16 ? 8 : 4;        // positions of a load there
+    if (a->keys >= chunk && (rows <= 64 || (double)heads * a->queries * a->keys <= NARROW_WORK)) {
         const int tk = a->dtype == VK_DTYPE_BF16 ? 128 : 64;
         kw = 0;
         d.tiles = (int)((rows + 15) / 16);

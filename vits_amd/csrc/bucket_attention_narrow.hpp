@@ -31,40 +31,50 @@ struct Narrow {
     __device__ __forceinline__ static int order(int m) { return 4 * (m & 3) + (m >> 2); }
     __device__ __forceinline__ static int krow(int n, int q4) { return sizeof(T) == 2 ? 32 * (n >> 3) + 8 * q4 + (n & 7) : 4 * n + q4; }
 
-    __device__ __forceinline__ static void load_keys(u32x4 (&k)[NK], const T* base, int64_t cstride, int d_real, int t0, int limit)
+    __device__ __forceinline__ static void load_keys(u32x4 (&k)[NK], const T* base, int64_t cstride, int d_real, int t0, int length)
     {
-        const int l = threadIdx.x & 63, q4 = l >> 4, col = E * order(l & 15);
-        if (t0 + TK <= limit && d_real == DP && cstride < (int64_t)(1 << 24)) {
+        const int l = threadIdx.x & 63, q4 = l >> 4, col = min(t0 + E * order(l & 15), length - E);
+        if (d_real == DP && cstride < (int64_t)(1 << 24)) {
             const unsigned lane = ((unsigned)(krow(0, 1) - krow(0, 0)) * (unsigned)q4 * (unsigned)cstride + (unsigned)col) * (unsigned)sizeof(T);
-            const char* p = (const char*)(base + t0);
+            const char* p = (const char*)base;
 #pragma unroll
             for (int n = 0; n < NK; ++n) __builtin_memcpy(&k[n], p + (int64_t)krow(n, 0) * cstride * (int64_t)sizeof(T) + lane, 16);
             return;
         }
+        // channels that are not there: any others, the queries are zero for them
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-            const int d = krow(n, q4);
-            const u32x4 c = load_chunk<T>(base + (int64_t)(d < d_real ? d : d_real - 1) * cstride, t0 + col, limit);
-            k[n] = d < d_real ? c : u32x4{0u, 0u, 0u, 0u};
-        }
+        for (int n = 0; n < NK; ++n) __builtin_memcpy(&k[n], base + (int64_t)min(krow(n, q4), d_real - 1) * cstride + col, 16);
     }
-    // Values: load (blk, r) of a lane is channel 16 blk + lane % 16, positions base + 4 E r + E (lane / 16).
-    __device__ __forceinline__ static void load_values(u32x4 (&v)[DP / 4], const T* base, int64_t cstride, int d_real, int t0, int limit)
+    // Values: load (blk, r) of a lane is channel 16 blk + lane % 16, positions base + 4 E r + E (lane / 16); zero at and
+    // behind `limit`, whatever lies there.
+    __device__ __forceinline__ static void load_values(u32x4 (&v)[DP / 4], const T* base, int64_t cstride, int d_real, int t0, int length, int limit)
     {
-        const int l = threadIdx.x & 63, row = l & 15, col = E * (l >> 4);
-        if (t0 + TK <= limit && d_real == DP && cstride < (int64_t)(1 << 24)) {
-            const unsigned lane = ((unsigned)row * (unsigned)cstride + (unsigned)col) * (unsigned)sizeof(T);
-            const char* p = (const char*)(base + t0);
+        const int l = threadIdx.x & 63, row = l & 15;
+        int col[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) col[r] = min(t0 + 4 * E * r + E * (l >> 4), length - E);
+        if (d_real == DP && cstride < (int64_t)(1 << 24)) {
+            const unsigned lane = (unsigned)row * (unsigned)cstride * (unsigned)sizeof(T);
+            const char* p = (const char*)base;
 #pragma unroll
             for (int n = 0; n < DP / 4; ++n)
-                __builtin_memcpy(&v[n], p + ((int64_t)(16 * (n >> 2)) * cstride + 4 * E * (n & 3)) * (int64_t)sizeof(T) + lane, 16);
-            return;
-        }
+                __builtin_memcpy(&v[n], p + (int64_t)(16 * (n >> 2)) * cstride * (int64_t)sizeof(T) + (lane + (unsigned)col[n & 3] * (unsigned)sizeof(T)), 16);
+        } else {
 #pragma unroll
-        for (int n = 0; n < DP / 4; ++n) {
-            const int d = 16 * (n >> 2) + row;
-            const u32x4 c = load_chunk<T>(base + (int64_t)(d < d_real ? d : d_real - 1) * cstride, t0 + 4 * E * (n & 3) + col, limit);
-            v[n] = d < d_real ? c : u32x4{0u, 0u, 0u, 0u};
+            for (int n = 0; n < DP / 4; ++n)
+                __builtin_memcpy(&v[n], base + (int64_t)min(16 * (n >> 2) + row, d_real - 1) * cstride + col[n & 3], 16);
+        }
+        if (t0 + TK <= limit) return;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            u32x4 keep;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (E == 4) keep[j] = col[r] + j < limit ? 0xffffffffu : 0u;
+                else keep[j] = (col[r] + 2 * j < limit ? 0xffffu : 0u) | (col[r] + 2 * j + 1 < limit ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int blk = 0; blk < DP / 16; ++blk) v[4 * blk + r] &= keep;
         }
     }
 };
@@ -158,7 +168,6 @@ void bucket_attention_narrow_kernel(Dev p)
     if (first < end) {
         u32x4 kr[N::NK], vr[DP / 4];
         const int t_first = first + wave * TK;
-        if (t_first < end) N::load_keys(kr, kg, p.kc, p.head_dim, t_first, end);
         // the rows' own queries: few, and read once
         typename N::frag qf[NQ];
         {
@@ -197,28 +206,35 @@ void bucket_attention_narrow_kernel(Dev p)
             right = p.bias[(int64_t)head * p.buckets + clampi(p.bucket_of[2 * p.far_], 0, p.buckets - 1)] * LOG2E;
         }
         __syncthreads();
-        for (int j0 = t_first; j0 < end; j0 += NWAVE * TK) {
-            N::load_values(vr, vg, p.vc, p.head_dim, j0, end);
+        // one round more than tiles: the first only requests keys
+        for (int j0 = t_first - NWAVE * TK; j0 < end; j0 += NWAVE * TK) {
+            const bool here = j0 >= t_first;
             f32x4v s[E];
+            if (here) {
+                N::load_values(vr, vg, p.vc, p.head_dim, j0, p.keys, end);
 #pragma unroll
-            for (int o = 0; o < E; ++o) s[o] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
-            narrow_scores<DP>(s, kr, qf);
-            if (j0 + NWAVE * TK < end) N::load_keys(kr, kg, p.kc, p.head_dim, j0 + NWAVE * TK, end);
+                for (int o = 0; o < E; ++o) s[o] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+                narrow_scores<DP>(s, kr, qf);
+            }
+            if (j0 + NWAVE * TK < end) N::load_keys(kr, kg, p.kc, p.head_dim, j0 + NWAVE * TK, p.keys);
+            if (!here) continue;
             const int side = bias_side(p, j0 - (it.start + i_hi), j0 + TK - 1 - (it.start + i_lo));
             const float flat = side == BIAS_LEFT ? left : side == BIAS_RIGHT ? right : 0.0f;
             const bool whole = j0 + TK <= end && !(p.causal && j0 + TK - 1 > it.start + i_lo);
             const int stop = p.causal ? min(end, pos + 1) : end;
             float mx = -__builtin_inff();
 #pragma unroll
-            for (int o = 0; o < E; ++o)
+            for (int r = 0; r < 4; ++r) {
+                const int first_j = j0 + 4 * E * r + E * q4, j8 = min(first_j, p.keys - E);     // see load_keys
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = j0 + 4 * E * r + E * q4 + o;
+                for (int o = 0; o < E; ++o) {
+                    const int j = j8 + o;
                     const float bias = side == BIAS_NEAR ? mine[clampi(j - pos, -p.far_, p.far_) + p.far_] : flat;
                     s[o][r] = fmaf(s[o][r], p.c, bias);
-                    if (!whole && j >= stop) s[o][r] = -__builtin_inff();
+                    if (!whole && (j < first_j || j >= stop)) s[o][r] = -__builtin_inff();
                     mx = fmaxf(mx, s[o][r]);
                 }
+            }
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             if (__any(mx > m + 8.0f)) {                     // as in the kernel for many rows: m follows in large steps

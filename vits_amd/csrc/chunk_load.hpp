@@ -35,13 +35,16 @@ __device__ __forceinline__ chunk_t load_chunk(const T* row, int t, int limit)
         __builtin_memcpy(&r, row + at, 16);
         return chunk_shift<E>(r, t - at < E ? t - at : E);
     }
-    if (limit <= 0) return r;
-    T tmp[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int at = t + e < limit ? t + e : limit - 1;
-        tmp[e] = t + e < limit ? row[at] : (T)0.0f;
+    // rows shorter than a chunk: a loop, so that this rare case costs few instructions
+    unsigned long long v[2] = {0, 0};
+#pragma unroll 1
+    for (int e = 0; e < limit - t; ++e) {
+        const T x = row[t + e];
+        unsigned bits = 0;
+        __builtin_memcpy(&bits, &x, sizeof(T));
+        const int pos = e * 8 * (int)sizeof(T);
+        v[0] |= pos < 64 ? (unsigned long long)bits << pos : 0;
+        v[1] |= pos >= 64 ? (unsigned long long)bits << (pos - 64) : 0;
     }
-    __builtin_memcpy(&r, tmp, 16);
-    return r;
+    return chunk_t{(unsigned)v[0], (unsigned)(v[0] >> 32), (unsigned)v[1], (unsigned)(v[1] >> 32)};
 }
