@@ -376,8 +376,8 @@ int vk_expand_prior(const float* durations, const float* m, const float* logs, f
  * A query without keys, and one at or behind query_lengths[b], gets out = 0 and lse = -inf.
  * bias [heads, buckets] fp32, bucket_of int32 [2 * max_distance + 1] (entries are clamped to the
  * buckets); has_bias = 0: no bias.  lse [B, heads, queries] fp32, dense.  Launches with few workgroups
- * share the keys out and join the shares through `workspace` (vk_bucket_attention_workspace_bytes; contents
- * irrelevant before and after; calls that may overlap in time need one each).
+ * share the keys out and join the shares through `workspace` (vk_bucket_attention_workspace_bytes, 16-byte aligned;
+ * contents irrelevant before and after; calls that may overlap in time need one each).  scale > 0.
  *
  * vk_bucket_attention_backward:  from q, k, v, bias, the forward's out and lse, and dout:
  *     p = exp(s - lse), ds_ij = p_ij (dout_i . v_j - dout_i . out_i)
@@ -421,7 +421,8 @@ int vk_bucket_attention_backward(const vk_bucket_attention_args* a, void* stream
  * v / sqrt(mean of squares + eps); statistics and parameters fp32, x, y, gate, h, n of type `dtype`.  n is taken of h
  * before h is rounded for storage.  gate: [B, C, T], or with gate_per_item one value per item and channel
  * (strides gate_bstride, gate_cstride).  Columns at or behind lengths[b] (NULL: none) are not read and written as 0.
- * h or n may be NULL (not wanted).  channels <= VK_BLOCK_NORM_MAX_CHANNELS, eps > 0.  Outputs must not overlap inputs.
+ * h or n may be NULL (not wanted).  channels <= VK_BLOCK_NORM_MAX_CHANNELS, eps > 0; an item's view spans less than 2^30
+ * elements.  Outputs must not overlap inputs.
  *
  * vk_block_norm_backward: dh, dn (either may be NULL: zero) -> dx, dy, dgate and the parameters' gradients (each may
  * be NULL if not wanted, but dx and, with y, dy), from h as stored, y, gate and the parameters:

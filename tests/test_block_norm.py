@@ -427,6 +427,7 @@ def test_c_entries_refuse_missing_pointers_overlaps_and_short_workspaces():
     assert F(x=0) == -1 and F(h=0, n=0) == -1 and F(h_cstride=99) == -1 and F(n_bstride=6399) == -1
     B = lambda **kw: L.vk_block_norm_backward(C.byref(_args(**kw)), None)
     assert B(dx=0) == -1 and B(dy=0) == -1 and B(dh=0, dn=0) == -1 and B(h=0) == -1 and B(gate=0) == -1 and B(scale=0) == -1
+    assert F(x_cstride=1 << 25) == -2 and B(dy_cstride=1 << 25) == -2            # an item of 2^30 elements or more
     assert B(dn=0) == -1 and B(dx_cstride=99) == -1 and B(dgate_cstride=99) == -1
     assert B() == -4
     a = _args()

@@ -239,6 +239,10 @@ def test_c_entries_refuse_missing_outputs_overlaps_and_short_workspaces():
     a.workspace, a.workspace_bytes = 4096, need - 4
     assert need > 0 and E(L.vk_bucket_attention_backward, a) == -4
     assert L.vk_bucket_attention_workspace_bytes(C.byref(_args(heads=3))) == -1
+    a.workspace, a.workspace_bytes = 4104, need
+    assert E(L.vk_bucket_attention_backward, a) == -1                          # not 16-byte aligned
+    for bad in (0.0, -1.0):
+        assert E(L.vk_bucket_attention, _args(scale=bad)) == -1
 
 
 def test_nothing_to_do_is_accepted():

@@ -124,7 +124,7 @@ def _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, 
 
 
 def _forward(q, k, v, bias, table, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
-    out = q.new_empty(q.shape)
+    out = native.empty_dense(q)
     lse = q.new_empty((q.shape[0], heads, q.shape[2]), dtype=torch.float32)
     native.bucket_attention(q, k, v, out, lse, bias, table, heads=heads, kv_heads=kv_heads, key_lengths=key_lengths,
                             query_lengths=query_lengths, query_start=query_start, causal=causal, scale=scale)
@@ -134,7 +134,7 @@ def _forward(q, k, v, bias, table, heads, kv_heads, key_lengths, query_lengths, 
 def _backward(dout, q, k, v, out, lse, bias, table, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
     # gradients of sums come expanded, results of other code in another order
     dout, out = (t if t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous() for t in (dout, out))
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dq, dk, dv = native.empty_dense(q), native.empty_dense(k), native.empty_dense(v)
     dbias = torch.empty_like(bias) if bias is not None else None
     native.bucket_attention_backward(dout, q, k, v, out, lse, dq, dk, dv, bias, table, dbias, heads=heads, kv_heads=kv_heads,
                                      key_lengths=key_lengths, query_lengths=query_lengths, query_start=query_start,
@@ -176,7 +176,7 @@ def bucket_attention(q, k, v, bias=None, buckets: RelativeBuckets | None = None,
     it), over j < key_lengths[b] and, with ``causal``, j <= pos_i.
 
     bias: float32 ``[heads, buckets.num_buckets]``, or None (no position bias).  key_lengths, query_lengths, query_start:
-    int64 ``[B]`` on the device, or None.  scale: 1 / sqrt(D) unless given.  Queries without a key and those at or behind
+    int64 ``[B]`` on the device, or None.  scale: 1 / sqrt(D) unless given, positive.  Queries without a key and those at or behind
     query_lengths[b] come out as zero; nothing behind a length is read, so padding may hold anything.  Serving a new
     token over a cache: Tq = 1, query_start = key_lengths - 1; the cache may be a view of a larger buffer.
 

@@ -79,8 +79,8 @@ def _check(like, y, gate, scale, post, pre, norm, eps, lengths):
 
 
 def _forward(x, y, gate, scale, post, pre, norm, eps, lengths):
-    h = x.new_empty(x.shape) if y is not None else None
-    n = x.new_empty(x.shape) if pre is not None else None
+    h = native.empty_dense(x) if y is not None else None
+    n = native.empty_dense(x) if pre is not None else None
     native.block_norm(x, y, h, n, gate=gate, scale=scale, post=post, pre=pre, norm=_NORMS[norm], eps=eps, lengths=lengths)
     return h, n
 
@@ -88,7 +88,7 @@ def _forward(x, y, gate, scale, post, pre, norm, eps, lengths):
 def _backward(dh, dn, h, y, gate, scale, post, pre, norm, eps, lengths):
     dh, dn = _dense(dh), _dense(dn)
     like = dh if dh is not None else dn
-    new = lambda t: t.new_empty(t.shape) if t is not None else None  # noqa: E731
+    new = lambda t: native.empty_dense(t) if t is not None else None  # noqa: E731
     dx, dy, dgate = new(like), new(y), new(gate)
     row = iter(like.new_empty((5, like.shape[1]), dtype=torch.float32).unbind(0))     # the parameters' gradients: one allocation
     par = lambda t: next(row) if t is not None else None  # noqa: E731
@@ -136,8 +136,8 @@ def block_norm(x, y=None, *, post=None, gate=None, scale=None, pre=None, norm: s
     _check(x, y, gate, scale, post, pre, norm, eps, lengths)
     w_post, b_post = post or (None, None)
     w_pre, b_pre = pre or (None, None)
-    given = [t for t in (x, y, gate, scale, w_post, b_post, w_pre, b_pre) if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, y, gate, scale, w_post, b_post, w_pre, b_pre)):
         _refuse_capture("block_norm")
         h, n = _BlockNorm.apply(x, y, gate, scale, w_post, b_post, w_pre, b_pre, norm, eps, lengths)
     else:

@@ -263,8 +263,8 @@ struct Dev {
     int batch, heads, group, head_dim, queries, keys, buckets, far_, causal;
     float scale, c;                 // c = scale * log2(e)
     int tiles, splits, per_split;   // row tiles of a head, shares of the other axis, its tiles per share
-    int units, spread, sort;        // (item, kv head) pairs; 1: a pair's workgroups on one XCD; 1: items by their work
-    int per_unit;
+    int units, spread, mix, sort;   // (item, kv head) pairs; a pair's workgroups on one XCD, its pairs side by side; items by their work
+    int per_unit, elem;             // bytes of an element
     float* part_o; float* part_ml;  // forward: partial results of the shares
     float* dbias; int kv_blocks, fold;   // backward: bias gradient; workgroups before those that sum it; the order of the dv ones
     float* delta; float* part_bias; // backward: row sums of out * dout; diagonal sums of the logit gradients
@@ -295,7 +295,8 @@ __device__ __forceinline__ Item uniform_item(const Dev& p, int b)
 
 // Workgroup -> (item, kv head, index within the pair).  Workgroups go round robin over the 8 XCDs; with `spread` all
 // workgroups of a pair share one XCD, so the keys and values of a head stay in that XCD's L2 (pairs are dealt back and
-// forth, 0..7 then 7..0).  With lengths, items go in the order of their work, the largest first: the XCDs then get
+// forth, 0..7 then 7..0).  With `mix` an XCD's pairs go on side by side instead of one after the other, so that the
+// longest workgroups of all of them come first.  With lengths, items go in the order of their work, the largest first: the XCDs then get
 // like shares, and what starts last is short.
 struct Place { int b, kvh, within; bool any; };
 __device__ __forceinline__ Place place(const Dev& p, int id)
@@ -304,9 +305,11 @@ __device__ __forceinline__ Place place(const Dev& p, int id)
     int unit;
     Place r;
     if (p.spread) {
-        const int slot = id >> 3, round = slot / p.per_unit;
+        const int slot = id >> 3, rounds = (p.units + 7) >> 3;
+        const int turn = slot / rounds;
+        const int round = p.mix ? (slot + turn) % rounds : slot / p.per_unit;
         unit = 8 * round + ((round & 1) ? 7 - (id & 7) : id & 7);
-        r.within = slot - round * p.per_unit;
+        r.within = p.mix ? turn : slot - round * p.per_unit;
     } else {
         unit = id / p.per_unit;
         r.within = id - unit * p.per_unit;

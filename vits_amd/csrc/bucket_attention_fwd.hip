@@ -293,11 +293,19 @@ int narrow_by_width(const Dev& d, hipStream_t st)
     }
 }
 
-#ifndef NARROW_WORK
-#define NARROW_WORK 6e5
-#endif
 // Which kernel (kw = 0: the one for few rows), queries per workgroup (128 or, with the waves in two key halves, 64)
 // and shares of the keys' length.
+//  * Few rows.  That kernel makes 16-row tiles over all rows of a kv head, the other 64-row tiles of one head each, and
+//    both read the keys and values once per tile.  In bf16 it pays where it makes fewer tiles (a token, 16 heads on one kv
+//    head, 8 x 8192 positions: 29 us against 63) or as many in a part of the chip (16 rows, 128 kv heads, 4096 positions:
+//    34 against 34; 512 heads of 1024: 45 against 33); in fp32, whose wide tiles take longer, up to twice as many (32
+//    rows, 128 heads: 77 against 102; 64 rows: 133 against 100) unless many short rows fill the chip (512 heads, 8 rows
+//    of 64 positions: 29 against 18).  And where few workgroups have little to do: eight bf16 heads of 256 positions,
+//    batch 2, 18 against 21; two fp32 heads of 301, 21 against 21, of 697, 33 against 22.
+//    A workgroup per CU: a token over 16 x 16384 positions took 207 us with shares for 256, 213 with shares for 512.
+//  * Two key halves: fp32 always (half the accumulators per wave; with one, two waves per SIMD do not fit), bf16 where
+//    128-row tiles would make no more than one workgroup per CU (8 heads of 128, 2048 positions: 46 us against 53; four
+//    times 8 heads of 96, 512 workgroups: 103 against 76) or stay half empty (one row, 512 heads of 1024: 33 against 41).
 void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& kw)
 {
     const int64_t heads = (int64_t)a->batch * a->heads;
@@ -305,18 +313,22 @@ void plan_forward(const vk_bucket_attention_args* a, Dev& d, int& kw)
     int64_t blocks, splits;
     int key_tiles, least;                                       // tiles of the key axis, the fewest in a share
     int row_tiles;
-    const int chunk = a->dtype == VK_DTYPE_BF16 ? 8 : 4;        // positions of a load there
-    if (a->keys >= chunk && (rows <= 64 || (double)heads * a->queries * a->keys <= NARROW_WORK)) {
-        const int tk = a->dtype == VK_DTYPE_BF16 ? 128 : 64;
+    const bool bf = a->dtype == VK_DTYPE_BF16;
+    const int chunk = bf ? 8 : 4;                               // positions of a load there
+    const int64_t units = (int64_t)a->batch * a->kv_heads, few = (rows + 15) / 16, wide = (int64_t)d.group * ((a->queries + 63) / 64);
+    const bool shared = bf ? few < wide || (few == wide && units * few <= 128)
+                           : few <= 2 * wide && (a->keys >= 512 || units * few <= 256);
+    if (a->keys >= chunk && (shared || (units * few <= 256 && a->keys <= 320))) {
+        const int tk = bf ? 128 : 64;
         kw = 0;
-        d.tiles = (int)((rows + 15) / 16);
+        d.tiles = (int)few;
         row_tiles = d.tiles;
-        blocks = (int64_t)a->batch * a->kv_heads * d.tiles;
+        blocks = units * few;
         key_tiles = (a->keys + tk - 1) / tk;
         least = NWAVE;
         splits = blocks == 0 ? 1 : (256 + blocks - 1) / blocks;
     } else {
-        kw = a->dtype == VK_DTYPE_F32 || heads * ((a->queries + 127) / 128) < 256 ? 2 : 1;
+        kw = !bf || a->queries <= 64 || heads * ((a->queries + 127) / 128) <= 256 ? 2 : 1;
         d.tiles = (a->queries + 128 / kw - 1) / (128 / kw);
         row_tiles = d.tiles * d.group;
         blocks = heads * d.tiles;

@@ -36,6 +36,7 @@ inline int vkba_check(const vk_bucket_attention_args* a, vkba::Dev& d, const cha
     if (a->has_bias && (a->buckets < 1 || a->max_distance < 1 || a->max_distance > VK_BUCKET_MAX_DISTANCE))
         return vkba_fail(VK_E_UNSUPPORTED, what, "bias needs at least one bucket and max_distance in 1..VK_BUCKET_MAX_DISTANCE");
     if (pointers) {
+        if ((uintptr_t)a->workspace & 15) return vkba_fail(VK_E_ARG, what, "workspace must be 16-byte aligned");
         if (a->has_bias && (!a->bias || !a->bucket_of)) return vkba_fail(VK_E_ARG, what, "null bias or bucket table");
         if (a->batch && a->queries && !a->q) return vkba_fail(VK_E_ARG, what, "null queries");
         if (a->batch && a->keys && (!a->k || !a->v)) return vkba_fail(VK_E_ARG, what, "null keys or values");
@@ -61,6 +62,7 @@ inline int vkba_check(const vk_bucket_attention_args* a, vkba::Dev& d, const cha
     d.scale = a->scale;
     d.c = a->scale * vkba::LOG2E;
     d.units = a->batch * a->kv_heads;
+    d.elem = a->dtype == VK_DTYPE_BF16 ? 2 : 4;
     return VK_OK;
 }
 
@@ -71,6 +73,10 @@ inline void vkba_place(vkba::Dev& d, int64_t per_unit)
     d.per_unit = (int)(per_unit > 0x7fffffff ? 0x7fffffff : per_unit);
     const int64_t rounds = (d.units + 7) / 8;
     d.spread = d.units >= 8 && rounds * 8 * 10 <= (int64_t)d.units * 11;
+    // causal: tiles differ in length most, and an XCD's pairs side by side (2048 causal positions: 128 -> 120 us) are
+    // worth it while their keys and values fit its 4 MiB of L2; padded batches alone lose by it (16 x 1001 fp32: 102 -> 121)
+    d.mix = d.spread && d.causal
+            && rounds * (int64_t)d.head_dim * 2 * (d.keys > d.queries ? d.keys : d.queries) * d.elem <= 4 << 20;
     d.sort = (d.nk || d.nq) && d.batch > 1 && d.batch <= 64;
 }
 inline int64_t vkba_blocks(const vkba::Dev& d)

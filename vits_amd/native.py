@@ -238,11 +238,11 @@ def lib():
         L.vk_dds_condition.argtypes = [C.POINTER(DdsArgs), C.c_void_p]
         L.vk_dds_coupling.argtypes = [C.POINTER(DdsArgs), C.c_void_p]
         for name in ("vk_bucket_attention", "vk_bucket_attention_backward"):
-            getattr(L, name).argtypes = [C.POINTER(BucketAttentionArgs), C.c_void_p]
-            getattr(L, name + "_workspace_bytes").argtypes = [C.POINTER(BucketAttentionArgs)]
+            getattr(L, name).argtypes = [C.c_void_p, C.c_void_p]           # packed bytes, or a reference to the mirror
+            getattr(L, name + "_workspace_bytes").argtypes = [C.c_void_p]
             getattr(L, name + "_workspace_bytes").restype = C.c_int64
-        L.vk_block_norm.argtypes = L.vk_block_norm_backward.argtypes = [C.POINTER(BlockNormArgs), C.c_void_p]
-        L.vk_block_norm_backward_workspace_bytes.argtypes = [C.POINTER(BlockNormArgs)]
+        L.vk_block_norm.argtypes = L.vk_block_norm_backward.argtypes = [C.c_void_p, C.c_void_p]
+        L.vk_block_norm_backward_workspace_bytes.argtypes = [C.c_void_p]
         L.vk_block_norm_backward_workspace_bytes.restype = C.c_int64
         L.vk_sizeof_args.argtypes = [C.c_int]
         L.vk_sizeof_args.restype = C.c_size_t
@@ -706,32 +706,50 @@ def _on_device(index, launch, *args):
         return launch(*args)
 
 
+def _packer(mirror):
+    """struct.Struct of a ctypes mirror: packing a tuple costs a third of filling the ctypes structure."""
+    import struct
+    code = {C.c_void_p: "P", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+    s = struct.Struct("@" + "".join(code[t] for _, t in mirror._fields_))
+    assert s.size <= C.sizeof(mirror) < s.size + 8          # the tail may be padded
+    return struct.Struct("@" + "".join(code[t] for _, t in mirror._fields_) + f"{C.sizeof(mirror) - s.size}x").pack
+
+
+_pack_bucket, _pack_norm = _packer(BucketAttentionArgs), _packer(BlockNormArgs)
+
+
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _view3(t):
     """(pointer, batch stride, channel stride) of a [B, C, T] view; zeros for None."""
     if t is None:
-        return None, 0, 0
+        return 0, 0, 0
     st = t.stride()
     return t.data_ptr(), st[0], st[1]
 
 
-def _run(entry, sizer, a, index, device, what, family, flops, nbytes, detail):
-    """Size the workspace (stream-ordered, from torch's allocator: a graph keeps its own) and launch."""
-    ref = C.byref(a)
+def empty_dense(t):
+    """A dense tensor of t's shape and type, not filled."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _run(entry, sizer, pack, head, tail, index, device, what, family, flops, nbytes, detail):
+    """Size the workspace (stream-ordered, from torch's allocator: a graph keeps its own) and launch.  The arguments are
+    ``head``, the workspace's pointer and size, ``tail``."""
+    args = pack(*head, 0, 0, *tail)
     if sizer is not None:
-        need = sizer(ref)
+        need = sizer(args)
         if need:
             check(min(need, 0), what)
             ws = torch.empty(need, device=device, dtype=torch.uint8)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), need
+            args = pack(*head, ws.data_ptr(), need, *tail)
     sp = torch._C._cuda_getCurrentRawStream(index)
     if LaunchTimer.active is None:
-        rc = entry(ref, sp)
+        rc = entry(args, sp)
     else:
-        rc = _timed(family, flops(), nbytes(), device, lambda: entry(ref, sp), detail())
+        rc = _timed(family, flops(), nbytes(), device, lambda: entry(args, sp), detail())
     if rc:
         check(rc, what)
 
@@ -742,14 +760,14 @@ def _bucket(name, q, k, v, out, lse, grads, bias, bucket_of, heads, kv_heads, ke
     dout, dq, dk, dv, dbias = grads
     B, Cq, Tq = q.shape
     Tk = k.shape[2]
-    a = BucketAttentionArgs(
-        *_view3(q), *_view3(k), *_view3(v), *_view3(out), lse.data_ptr(), *_view3(dout), *_view3(dq), *_view3(dk), *_view3(dv),
-        _ptr(dbias), _ptr(bias), _ptr(bucket_of), _ptr(key_lengths), _ptr(query_lengths), _ptr(query_start), None, 0,
-        B, heads, kv_heads, Cq // heads, Tq, Tk, bias is not None, bias.shape[1] if bias is not None else 0,
-        bucket_of.shape[0] // 2 if bias is not None else 0, bool(causal), DTYPES[q.dtype], scale)
+    head = (*_view3(q), *_view3(k), *_view3(v), *_view3(out), lse.data_ptr(), *_view3(dout), *_view3(dq), *_view3(dk), *_view3(dv),
+            _ptr(dbias), _ptr(bias), _ptr(bucket_of), _ptr(key_lengths), _ptr(query_lengths), _ptr(query_start))
+    tail = (B, heads, kv_heads, Cq // heads, Tq, Tk, bias is not None, bias.shape[1] if bias is not None else 0,
+            bucket_of.shape[0] // 2 if bias is not None else 0, bool(causal), DTYPES[q.dtype], scale)
     L, device = lib(), q.device
     backward = dout is not None
-    _on_device(device.index, _run, getattr(L, name), getattr(L, name + "_workspace_bytes"), a, device.index, device, name, name[3:],
+    _on_device(device.index, _run, getattr(L, name), getattr(L, name + "_workspace_bytes"), _pack_bucket, head, tail, device.index,
+               device, name, name[3:],
                lambda: (10.0 if backward else 4.0) * B * Cq * Tq * Tk,
                lambda: (2 if backward else 1) * q.element_size() * (2 * q.numel() + k.numel() + v.numel()),
                lambda: f"B{B} H{heads}/{kv_heads} D{Cq // heads} Tq{Tq} Tk{Tk}")
@@ -775,13 +793,13 @@ def _norm(name, like, x, y, gate, scale, post, pre, h, n, lengths, grads, norm, 
     dh, dn, dx, dy, dgate, dscale, dpost, dpre = grads
     B, Cn, T = like.shape
     none = (None, None)
-    a = BlockNormArgs(
-        *_view3(x), *_view3(y), *_view3(gate), _ptr(scale), *map(_ptr, post or none), *map(_ptr, pre or none), *_view3(h), *_view3(n),
-        _ptr(lengths), *_view3(dh), *_view3(dn), *_view3(dx), *_view3(dy), *_view3(dgate), _ptr(dscale), *map(_ptr, dpost or none),
-        *map(_ptr, dpre or none), None, 0, B, Cn, T, gate is not None and gate.shape[2] == 1 and T != 1, norm, DTYPES[like.dtype], eps)
+    head = (*_view3(x), *_view3(y), *_view3(gate), _ptr(scale), *map(_ptr, post or none), *map(_ptr, pre or none), *_view3(h),
+            *_view3(n), _ptr(lengths), *_view3(dh), *_view3(dn), *_view3(dx), *_view3(dy), *_view3(dgate), _ptr(dscale),
+            *map(_ptr, dpost or none), *map(_ptr, dpre or none))
+    tail = B, Cn, T, gate is not None and gate.shape[2] == 1 and T != 1, norm, DTYPES[like.dtype], eps
     L, device = lib(), like.device
-    _on_device(device.index, _run, getattr(L, name), L.vk_block_norm_backward_workspace_bytes if dx is not None else None, a,
-               device.index, device, name, name[3:], lambda: (20.0 if dx is None else 40.0) * like.numel(),
+    _on_device(device.index, _run, getattr(L, name), L.vk_block_norm_backward_workspace_bytes if dx is not None else None, _pack_norm,
+               head, tail, device.index, device, name, name[3:], lambda: (20.0 if dx is None else 40.0) * like.numel(),
                lambda: like.element_size() * sum(t.numel() for t in (x, y, gate, h, n, dh, dn, dx, dy, dgate) if t is not None),
                lambda: f"B{B} C{Cn} T{T}")
 
