@@ -294,6 +294,23 @@ def test_many_workgroups(dtype):
         assert_within(name, g, ref[name])
 
 
+SHARED = [
+    (1, 16, 1, 128, 300, 300, (32, 128, False), True, None, None, None),          # queries of 16 heads in shares, causal
+    (2, 2, 2, 96, 500, 333, BIDIR, False, [333, 0], [500, 411], [3, 0]),          # shares of one head's queries, an empty item
+    (1, 8, 2, 64, 257, 255, SMALL, False, [251], [130], None),                    # shares beyond the length
+    (3, 6, 2, 72, 129, 129, None, True, [129, 1, 64], [129, 1, 64], None),
+    (33, 4, 4, 32, 1, 70, (32, 128, False), True, [70 - i for i in range(33)], None, [69 - i for i in range(33)]),   # tokens of many heads
+    (1, 2, 2, 64, 60, 1500, BIDIR, False, [1489], None, [700]),                   # few rows, long: wide tiles, shared keys
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("case", SHARED, ids=[f"B{c[0]}H{c[1]}-{c[2]}D{c[3]}T{c[4]}-{c[5]}" for c in SHARED])
+def test_shares_of_the_other_axis(case, dtype):
+    test_forward_and_backward(case, dtype)
+
+
 @gpu
 @pytest.mark.parametrize("Tq,Tk", [(0, 5), (5, 0), (0, 0)])
 def test_empty_lengths(Tq, Tk):

@@ -252,6 +252,18 @@ __device__ __forceinline__ void flip(float (&f)[N], bool neg)
 
 // Row (position within 32) of accumulator register r in lane half h.
 __device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+// Accumulators (32 channels x 32 positions each), times f, to rows of a tensor; g: channel 0, this lane's position.
+template <typename T, int NB>
+__device__ __forceinline__ void store_rows(T* g, int64_t cstride, int d_real, const f32x16 (&x)[NB], int h, bool valid, float f)
+{
+#pragma unroll
+    for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = 32 * blk + acc_row(r, h);
+            if (d < d_real) g[(int64_t)d * cstride] = (T)(valid ? x[blk][r] * f : 0.0f);
+        }
+}
 
 struct Dev {
     const void* q; const void* k; const void* v; const void* o; const void* dout;
@@ -267,6 +279,7 @@ struct Dev {
     int per_unit, elem;             // bytes of an element
     float* part_o; float* part_ml;  // forward: partial results of the shares
     float* dbias; int kv_blocks, fold;   // backward: bias gradient; workgroups before those that sum it; the order of the dv ones
+    int shares; float* part_kv;     // backward: shares of the queries, their sums for dk and dv
     float* delta; float* part_bias; // backward: row sums of out * dout; diagonal sums of the logit gradients
 };
 

@@ -19,12 +19,16 @@ struct Shape {
     static constexpr bool BF = sizeof(T) == 2;
     static constexpr bool SPLIT = BF && DP > 96;
     static constexpr int MIN_WAVES = BF || DP <= 64 ? 2 : 1;
-    // the next tile is loaded into registers while the present one is computed, unless they make the second wave
-    static constexpr bool AHEAD = BF || MIN_WAVES == 1;
+    // the next tile is loaded into registers while the present one is computed, unless that makes the rest spill (bf16,
+    // 8 x 8 heads of 96, 2048 positions: 594 us with, 533 without; 16 heads of 128 on 4, 1024 positions: 131, 110; the
+    // 128-channel kernel with tiles of 32 has room) or, fp32, takes the second wave
+    static constexpr bool AHEAD = BF ? DP <= 64 || (DP > 96 && KW == 1) : MIN_WAVES == 1;
     static constexpr int KT_DQ = BF && DP > 96 && KW == 1 ? 32 : 64, KT_DKV = KT_DQ;
     static constexpr int OWN = Tile<T, DP, 64>::BYTES;                  // image of 64 of the workgroup's own rows
     static constexpr int IMAGES = 2 * OWN;                              // as large as two tiles
 };
+
+__host__ __device__ inline int64_t kv_elements(const Dev& p) { return (int64_t)p.batch * (p.heads / p.group) * p.head_dim * p.keys; }
 
 constexpr int DGP = 33;         // pitch of a wave's 32 x 32 block of logit gradients
 
@@ -202,14 +206,7 @@ void bucket_dq_kernel(Dev p)
                 for (int r = 0; r < 16; ++r) acc[blk][r] += red[(32 * blk + acc_row(r, h)) * 32];
     }
     if (qi < p.queries && kw == 0) {
-        T* dqg = (T*)p.dq + (int64_t)b * p.dqb + hd * p.dqc + qi;
-#pragma unroll
-        for (int blk = 0; blk < DP / 32; ++blk)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int d = 32 * blk + acc_row(r, h);
-                if (d < p.head_dim) dqg[(int64_t)d * p.dqc] = (T)(valid ? acc[blk][r] * (sgn * p.scale) : 0.0f);
-            }
+        store_rows((T*)p.dq + (int64_t)b * p.dqb + hd * p.dqc + qi, p.dqc, p.head_dim, acc, h, valid, sgn * p.scale);
     }
     if (p.bias) {
         if (lse2 < __builtin_inff()) {                      // what the rounding of (bias - lse2) and of lse2 left out
@@ -254,7 +251,8 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
     const int l = threadIdx.x & 63, h = l >> 5, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int cw = wave / KW, kw = wave % KW;
     const int within = reverse ? p.per_unit - 1 - at.within : at.within;
-    const int kt0 = within * CW * 32, jb = kt0 + cw * 32, j = jb + (l & 31);
+    const int share = within % p.shares;
+    const int kt0 = within / p.shares * CW * 32, jb = kt0 + cw * 32, j = jb + (l & 31);
     const bool valid = j < it.nk;
     const int64_t hd = (int64_t)kvh * p.head_dim;
 
@@ -279,7 +277,8 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
     int q_first = 0;
     if (p.causal) q_first = clampi(kt0 - it.start, 0, it.nq) / KT * KT;
     const int tiles = kt0 < it.nk ? (it.nq - q_first + KT - 1) / KT : 0;
-    const int steps = tiles > 0 ? tiles * p.group : 0;
+    const int steps = tiles > 0 ? tiles * p.group : 0;                          // (head, query tile), of which this share has
+    const int first = (int)((int64_t)steps * share / p.shares), last = (int)((int64_t)steps * (share + 1) / p.shares);
 
     Tile<T, DP, KT> qt, dt;
     float stat = 0.0f;
@@ -295,8 +294,8 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
             stat = i < it.nq ? src[row + i] : threadIdx.x < KT ? -__builtin_inff() : 0.0f;
         }
     };
-    if (S::AHEAD && steps > 0) fetch(0);
-    for (int step = 0; step < steps; ++step) {
+    if (S::AHEAD && first < last) fetch(first);
+    for (int step = first; step < last; ++step) {
         const int g = step / tiles, tile = step - g * tiles, i0 = q_first + tile * KT;
         if constexpr (!S::AHEAD) fetch(step);
         __syncthreads();
@@ -304,9 +303,9 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
         dt.store(dim);
         if (threadIdx.x < KT) st[threadIdx.x] = stat == -__builtin_inff() ? __builtin_inff() : stat * LOG2E;    // no keys: all probabilities 0
         else if (threadIdx.x < 2 * KT) st[threadIdx.x] = -stat;
-        if (tile == 0) stage_bias(tab, p, kvh * p.group + g);
+        if (tile == 0 || step == first) stage_bias(tab, p, kvh * p.group + g);
         __syncthreads();
-        if (S::AHEAD && step + 1 < steps) fetch(step + 1);
+        if (S::AHEAD && step + 1 < last) fetch(step + 1);
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c0 = 32 * (kw * NS + i), is = i0 + c0, pos0 = it.start + is;     // this block's queries
@@ -339,7 +338,7 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
         }
     }
     float* red = reinterpret_cast<float*>(lds) + cw * DP * 32 + (l & 31);
-    auto finish = [&](f32x16 (&x)[DP / 32], void* out, int64_t bstride, int64_t cstride, float scale) {
+    auto finish = [&](f32x16 (&x)[DP / 32], float* part, void* out, int64_t bstride, int64_t cstride, float scale) {
         if constexpr (KW == 2) {
             __syncthreads();
             if (kw == 1)
@@ -355,17 +354,15 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
                     for (int r = 0; r < 16; ++r) x[blk][r] += red[(32 * blk + acc_row(r, h)) * 32];
         }
         if (j >= p.keys || kw != 0) return;
-        T* g = (T*)out + (int64_t)b * bstride + hd * cstride + j;
-#pragma unroll
-        for (int blk = 0; blk < DP / 32; ++blk)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int d = 32 * blk + acc_row(r, h);
-                if (d < p.head_dim) g[(int64_t)d * cstride] = (T)(valid ? x[blk][r] * scale : 0.0f);
-            }
+        if (p.shares > 1) {
+            float* g = part + (((int64_t)share * p.batch + b) * (p.heads / p.group) * p.head_dim + hd) * p.keys + j;
+            store_rows(g, p.keys, p.head_dim, x, h, valid, scale);
+        } else {
+            store_rows((T*)out + (int64_t)b * bstride + hd * cstride + j, cstride, p.head_dim, x, h, valid, scale);
+        }
     };
-    if constexpr (DK) finish(dk, p.dk, p.dkb, p.dkc, p.scale);
-    if constexpr (DV) finish(dv, p.dv, p.dvb, p.dvc, 1.0f);
+    if constexpr (DK) finish(dk, p.part_kv, p.dk, p.dkb, p.dkc, p.scale);
+    if constexpr (DV) finish(dv, p.part_kv + p.shares * kv_elements(p), p.dv, p.dvb, p.dvc, 1.0f);
 }
 
 // dbias[h, c] = sum of the diagonal sums whose offset falls into bucket c, over all workgroups of head h, in 64 bits
@@ -418,6 +415,30 @@ void bucket_dkv_kernel(Dev p)
     dbias_of_head(p, id - p.kv_blocks, lds);
 }
 
+// Sum of the shares of dk and dv; a workgroup has 1024 keys of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void bucket_kv_sum_kernel(Dev p)
+{
+    const int per_row = (p.keys + 1023) / 1024, rows_of_item = p.heads / p.group * p.head_dim;
+    const int64_t rows = (int64_t)p.batch * rows_of_item, n = kv_elements(p);
+    int64_t row = blockIdx.x / per_row;
+    const int j0 = (int)(blockIdx.x - row * per_row) * 1024 + (int)threadIdx.x;
+    const bool is_v = row >= rows;
+    const float* part = p.part_kv + (is_v ? p.shares * n : 0);
+    if (is_v) row -= rows;
+    const int64_t b = row / rows_of_item, c = row - b * rows_of_item;
+    T* out = is_v ? (T*)p.dv + b * p.dvb + c * p.dvc : (T*)p.dk + b * p.dkb + c * p.dkc;
+    part += row * p.keys;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 256 * i;
+        if (j >= p.keys) return;
+        float x = 0.0f;
+        for (int s = 0; s < p.shares; ++s) x += part[s * n + j];
+        out[j] = (T)x;
+    }
+}
+
 template <typename T, int DP, int KW>
 int launch_both(Dev d, hipStream_t st)
 {
@@ -432,7 +453,7 @@ int launch_both(Dev d, hipStream_t st)
         int rc = vkba_launch<bucket_dq_kernel<T, DP, KW>>(d, vkba_blocks(d), lds, st, what);
         if (rc != VK_OK) return rc;
     }
-    vkba_place(d, (d.keys + ROWS - 1) / ROWS);
+    vkba_place(d, (int64_t)(d.keys + ROWS - 1) / ROWS * d.shares);
     const int64_t blocks = d.keys > 0 ? vkba_blocks(d) : 0;
     if (blocks > 0x7fffffff) return vkba_fail(VK_E_UNSUPPORTED, what, "too many workgroups");
     d.kv_blocks = (int)blocks;
@@ -440,8 +461,10 @@ int launch_both(Dev d, hipStream_t st)
     // those of dv come in the other order, so that a CU gets a long and a short one
     d.fold = d.causal && 2 * blocks <= 512;
     const size_t need = S::IMAGES + 2 * S::KT_DKV * 4 + vkba_table_bytes(d);
-    return vkba_launch<bucket_dkv_kernel<T, DP, KW>>(d, (S::SPLIT ? 2 : 1) * blocks + (d.bias ? d.heads : 0),
-                                                     need > offsets * 8 ? need : offsets * 8, st, what);
+    int rc = vkba_launch<bucket_dkv_kernel<T, DP, KW>>(d, (S::SPLIT ? 2 : 1) * blocks + (d.bias ? d.heads : 0),
+                                                       need > offsets * 8 ? need : offsets * 8, st, what);
+    if (rc != VK_OK || d.shares == 1) return rc;
+    return vkba_launch<bucket_kv_sum_kernel<T>>(d, 2 * (kv_elements(d) / d.keys) * ((d.keys + 1023) / 1024), 0, st, what);
 }
 
 template <typename T, int KW>
@@ -465,10 +488,29 @@ int64_t parts_of_head(const vk_bucket_attention_args* a)
     const int rows = 128 / key_waves(a);
     return (int64_t)a->batch * ((a->queries + rows - 1) / rows);
 }
+// Shares of the queries (of all heads of the group), each with workgroups of its own for dk and dv; a third launch sums
+// them.  Where the workgroups would fill less than half of the chip (one bf16 head of 128 shared by 16, 2048 causal
+// positions: 1510 us without, 233 with shares; two fp32 heads of 96, 697 positions: 177, 130; not above: four
+// times 8 bf16 heads of 64, 2048 positions, 512 workgroups: 156, 170).  With `causal` also where each walks far: the
+// first keys have nearly twice the mean work, and the chip waits for them (4095 positions, 16 heads on 4, batch 2,
+// 512 workgroups: 755 us for dk and dv without, 602 + 20 with two shares and their sum).
+int key_shares(const vk_bucket_attention_args* a)
+{
+    const int group = a->kv_heads > 0 ? a->heads / a->kv_heads : 1, rows = 128 / key_waves(a);
+    const bool split = a->dtype == VK_DTYPE_BF16 && a->head_dim > 96;
+    const int64_t blocks = (int64_t)a->batch * a->kv_heads * ((a->keys + rows - 1) / rows) * (split ? 2 : 1);
+    const int64_t steps = (int64_t)group * ((a->queries + 63) / 64), slots = a->dtype == VK_DTYPE_F32 && a->head_dim > 64 ? 256 : 512;
+    const int64_t target = a->causal && steps >= 64 ? 1024 : blocks < slots / 2 ? slots : 0;
+    if (blocks == 0 || blocks >= target) return 1;
+    const int64_t want = (target + blocks - 1) / blocks, most = steps / 2;
+    return (int)(want < most ? want : most < 1 ? 1 : most);
+}
 int64_t workspace_floats(const vk_bucket_attention_args* a)
 {
     const int64_t delta = (int64_t)a->batch * a->heads * a->queries;
-    return delta + (a->has_bias ? parts_of_head(a) * a->heads * (2 * (int64_t)a->max_distance + 1) : 0);
+    const int64_t shares = key_shares(a);
+    const int64_t kv = shares > 1 ? 2 * shares * a->batch * a->kv_heads * a->head_dim * a->keys : 0;
+    return delta + kv + (a->has_bias ? parts_of_head(a) * a->heads * (2 * (int64_t)a->max_distance + 1) : 0);
 }
 
 }  // namespace
@@ -498,7 +540,9 @@ extern "C" int vk_bucket_attention_backward(const vk_bucket_attention_args* a, v
     if (need > 0 && (!a->workspace || a->workspace_bytes < need))
         return vkba_fail(VK_E_WORKSPACE, what, "workspace smaller than vk_bucket_attention_backward_workspace_bytes");
     d.delta = (float*)a->workspace;
-    d.part_bias = d.delta + (int64_t)a->batch * a->heads * a->queries;
+    d.shares = key_shares(a);
+    d.part_kv = d.delta + (int64_t)a->batch * a->heads * a->queries;
+    d.part_bias = d.part_kv + (d.shares > 1 ? 2 * d.shares * kv_elements(d) : 0);
     d.dbias = a->dbias;
     hipStream_t st = (hipStream_t)stream;
     if (key_waves(a) == 2) return a->dtype == VK_DTYPE_BF16 ? by_width<__bf16, 2>(d, st) : by_width<float, 2>(d, st);
