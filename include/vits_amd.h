@@ -377,7 +377,7 @@ int vk_expand_prior(const float* durations, const float* m, const float* logs, f
  * bias [heads, buckets] fp32, bucket_of int32 [2 * max_distance + 1] (entries are clamped to the
  * buckets); has_bias = 0: no bias.  lse [B, heads, queries] fp32, dense.  Launches with few workgroups
  * share the keys out and join the shares through `workspace` (vk_bucket_attention_workspace_bytes, 16-byte aligned;
- * contents irrelevant before and after; calls that may overlap in time need one each).  scale > 0.
+ * contents irrelevant before and after; calls that may overlap in time need one each).  scale > 0, batch * heads < 2^23.
  *
  * vk_bucket_attention_backward:  from q, k, v, bias, the forward's out and lse, and dout:
  *     p = exp(s - lse), ds_ij = p_ij (dout_i . v_j - dout_i . out_i)

@@ -428,6 +428,8 @@ def test_c_entries_refuse_missing_pointers_overlaps_and_short_workspaces():
     B = lambda **kw: L.vk_block_norm_backward(C.byref(_args(**kw)), None)
     assert B(dx=0) == -1 and B(dy=0) == -1 and B(dh=0, dn=0) == -1 and B(h=0) == -1 and B(gate=0) == -1 and B(scale=0) == -1
     assert F(x_cstride=1 << 25) == -2 and B(dy_cstride=1 << 25) == -2            # an item of 2^30 elements or more
+    many = dict(batch=1 << 24, length=1, channels=1)                            # more workgroups than a grid holds
+    assert F(**many) == -2 and B(**many, workspace=4096, workspace_bytes=1 << 40) == -2
     assert B(dn=0) == -1 and B(dx_cstride=99) == -1 and B(dgate_cstride=99) == -1
     assert B() == -4
     a = _args()

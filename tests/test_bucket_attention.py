@@ -239,6 +239,7 @@ def test_c_entries_refuse_missing_outputs_overlaps_and_short_workspaces():
     a.workspace, a.workspace_bytes = 4096, need - 4
     assert need > 0 and E(L.vk_bucket_attention_backward, a) == -4
     assert L.vk_bucket_attention_workspace_bytes(C.byref(_args(heads=3))) == -1
+    assert L.vk_bucket_attention_workspace_bytes(C.byref(_args(batch=1 << 20, heads=16, kv_heads=2))) == -2    # more heads than a grid holds
     a.workspace, a.workspace_bytes = 4104, need
     assert E(L.vk_bucket_attention_backward, a) == -1                          # not 16-byte aligned
     for bad in (0.0, -1.0):

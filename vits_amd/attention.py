@@ -181,7 +181,7 @@ def bucket_attention(q, k, v, bias=None, buckets: RelativeBuckets | None = None,
     token over a cache: Tq = 1, query_start = key_lengths - 1; the cache may be a view of a larger buffer.
 
     Returns out ``[B, heads * D, Tq]``, with ``return_lse`` also the log-sum-exp of the logits ``[B, heads, Tq]`` (-inf
-    where there is no key), which ``bucket_attention_backward`` takes."""
+    where there is no key), which ``bucket_attention_backward`` takes and which carries no gradient."""
     kv_heads, scale, table = _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, query_start, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (bias is not None and bias.requires_grad)):

@@ -565,7 +565,7 @@ template <typename T, int LT, int NW, int R>
 int launch(const NDev& d, bool backward, hipStream_t st, const char* what)
 {
     const int64_t blocks = ((int64_t)d.a.batch * d.windows + 7) / 8 * 8;       // see Spot
-    if (blocks > 0x7fffffff) return fail(VK_E_UNSUPPORTED, what, "too many workgroups");
+    if (blocks * 64 * NW > 0xffffffffLL) return fail(VK_E_UNSUPPORTED, what, "too many workgroups");     // the limit of a grid, in threads
     const size_t lds = (NW * LT * Pack<T>::E + P_COUNT * (size_t)d.a.channels) * 4;
     return backward ? launch_kernel<block_norm_backward_kernel<T, LT, NW, R>>(d, blocks, 64 * NW, lds, st, what)
                     : launch_kernel<block_norm_kernel<T, LT, NW, R>>(d, blocks, 64 * NW, lds, st, what);
@@ -624,6 +624,8 @@ extern "C" int vk_block_norm_backward(const vk_block_norm_args* a, void* stream)
     int rc = check(a, what, true);
     if (rc != VK_OK) return rc;
     const Plan pl = plan_of(a);
+    const bool gates = a->dgate && a->gate_per_item;
+    if (gates && a->batch > 65530) return fail(VK_E_UNSUPPORTED, what, "a gate per item: batch > 65530");
     const int64_t need = workspace_floats(a) * 4;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need))
         return fail(VK_E_WORKSPACE, what, "workspace smaller than vk_block_norm_backward_workspace_bytes");
@@ -634,9 +636,7 @@ extern "C" int vk_block_norm_backward(const vk_block_norm_args* a, void* stream)
         rc = a->dtype == VK_DTYPE_BF16 ? by_shape<__bf16>(d, pl, true, st, what) : by_shape<float>(d, pl, true, st, what);
         if (rc != VK_OK) return rc;
     }
-    const bool gates = a->dgate && a->gate_per_item;
     if (!a->dw_pre && !a->db_pre && !a->dscale && !a->dw_post && !a->db_post && !gates) return VK_OK;
-    if (a->batch > 65530) return fail(VK_E_UNSUPPORTED, what, "batch > 65530");
     dim3 grid((unsigned)((a->channels + SUM_C - 1) / SUM_C), (unsigned)(5 + (gates ? a->batch : 0)));
     if (a->dtype == VK_DTYPE_BF16) hipLaunchKernelGGL(block_norm_sums_kernel<__bf16>, grid, dim3(SUM_C * SUM_P), 0, st, d);
     else hipLaunchKernelGGL(block_norm_sums_kernel<float>, grid, dim3(SUM_C * SUM_P), 0, st, d);

@@ -31,6 +31,7 @@ inline int vkba_check(const vk_bucket_attention_args* a, vkba::Dev& d, const cha
         return vkba_fail(VK_E_ARG, what, "bad batch, length or head count (heads must be a multiple of kv_heads)");
     if (a->dtype != VK_DTYPE_F32 && a->dtype != VK_DTYPE_BF16) return vkba_fail(VK_E_UNSUPPORTED, what, "dtype must be VK_DTYPE_F32 or VK_DTYPE_BF16");
     if (a->head_dim < 1 || a->head_dim > VK_BUCKET_MAX_HEAD_DIM) return vkba_fail(VK_E_UNSUPPORTED, what, "head_dim must be 1..128");
+    if ((int64_t)a->batch * a->heads > 0x7fffff) return vkba_fail(VK_E_UNSUPPORTED, what, "batch x heads beyond 2^23");
     if (a->queries > VK_BUCKET_MAX_LENGTH || a->keys > VK_BUCKET_MAX_LENGTH) return vkba_fail(VK_E_UNSUPPORTED, what, "length beyond VK_BUCKET_MAX_LENGTH");
     if (!(a->scale > 0.0f && a->scale < 1e30f)) return vkba_fail(VK_E_ARG, what, "scale must be positive and finite");
     if (a->has_bias && (a->buckets < 1 || a->max_distance < 1 || a->max_distance > VK_BUCKET_MAX_DISTANCE))
@@ -90,7 +91,7 @@ template <auto KERNEL>
 int vkba_launch(const vkba::Dev& d, int64_t blocks, size_t lds, hipStream_t st, const char* what)
 {
     if (blocks <= 0) return VK_OK;
-    if (blocks > 0x7fffffff) return vkba_fail(VK_E_UNSUPPORTED, what, "too many workgroups");
+    if (blocks * vkba::NTHR > 0xffffffffLL) return vkba_fail(VK_E_UNSUPPORTED, what, "too many workgroups");    // the limit of a grid, in threads
     static std::atomic<unsigned long long> raised{0};
     hipError_t e = vk_allow_lds(KERNEL, lds, raised);
     if (e != hipSuccess) return vkba_fail(VK_E_LAUNCH, what, hipGetErrorString(e));
