@@ -9,6 +9,9 @@
 // memory, the statistics need no second one.  Lanes lie along time (one 16-byte access per lane and row), the
 // channels are spread over the other lanes and the waves; column sums meet through LDS.
 // Bound by memory: forward reads x, y, gate and writes h, n; backward reads dh, dn, h, y, gate, writes dx, dy, dgate.
+// fp32, 32 x 256 x 2048: 75 us (4.5 TB/s), backward 136 us (3.9 TB/s).  bf16, 8 x 1024 x 4096, gate per item: 93 us (2.9 TB/s);
+// 8 x up to 2047 x 1024 backward 131 us (1.6 TB/s): that many channels leave one workgroup per CU, whose loads and
+// arithmetic alternate.
 #include <hip/hip_runtime.h>
 #include <atomic>
 #include <stdint.h>
@@ -535,13 +538,18 @@ int check(const vk_block_norm_args* a, const char* what, bool backward)
 
 // A workgroup's window: LT lanes of 16 bytes along time, NW waves, R channels per thread, so (64 / LT) * NW * R
 // channels.  Eight lanes make 128-byte accesses, a whole cache line; narrower windows hold more channels and
-// make more workgroups.
+// make more workgroups.  Few channels per thread keep several workgroups on a CU, so that one loads while another computes:
+// eight waves of four rather than four of eight (fp32 backward, 32 x 256 x 2048: 136 us against 144; 64 x 192 x 862: 99,
+// 113), and in bf16, whose lanes hold eight columns, 129..256 channels in half as wide windows (160 channels, 16 x 4095:
+// 79 us against 84 and, with four waves of eight, 112; in fp32 not: 32 x 256 x 2048 150 against 136; nor from 512 channels on,
+// where rows of 32 bytes cost more than they gain: 8 x 1024 x 2047 147 against 124).
 struct Plan { int lt, nw, r; };
 Plan plan_of(const vk_block_norm_args* a)
 {
-    static constexpr int kShapes[3][2] = {{4, 4}, {4, 8}, {8, 8}};
+    static constexpr int kShapes[3][2] = {{4, 4}, {8, 4}, {8, 8}};
     const int e = a->dtype == VK_DTYPE_BF16 ? 8 : 4;
     Plan pl{8, 8, 8};
+    if (e == 8 && a->channels > 128 && a->channels <= 256) pl.lt = 4;
     while (pl.lt > 1 && (64 / pl.lt) * kShapes[2][0] * kShapes[2][1] < a->channels) pl.lt >>= 1;
     // fewer than 256 workgroups: narrower windows spread over more CUs
     while (pl.lt > 1 && (int64_t)a->batch * ((a->length + pl.lt * e - 1) / (pl.lt * e)) < 256) pl.lt >>= 1;
@@ -574,7 +582,9 @@ template <typename T, int NW, int R>
 int by_window(const NDev& d, int lt, bool backward, hipStream_t st, const char* what)
 {
     switch (lt) {
-    case 8: return launch<T, 8, NW, R>(d, backward, st, what);
+    case 8:
+        if constexpr (!(Pack<T>::E == 8 && NW == 8 && R == 4)) return launch<T, 8, NW, R>(d, backward, st, what);
+        return fail(VK_E_UNSUPPORTED, what, "no such window");      // plan_of takes four lanes there
     case 4: return launch<T, 4, NW, R>(d, backward, st, what);
     case 2: return launch<T, 2, NW, R>(d, backward, st, what);
     default: return launch<T, 1, NW, R>(d, backward, st, what);
@@ -583,8 +593,8 @@ int by_window(const NDev& d, int lt, bool backward, hipStream_t st, const char* 
 template <typename T>
 int by_shape(const NDev& d, const Plan& pl, bool backward, hipStream_t st, const char* what)
 {
-    if (pl.nw == 4 && pl.r == 4) return by_window<T, 4, 4>(d, pl.lt, backward, st, what);
-    return pl.nw == 4 ? by_window<T, 4, 8>(d, pl.lt, backward, st, what) : by_window<T, 8, 8>(d, pl.lt, backward, st, what);
+    if (pl.nw == 4) return by_window<T, 4, 4>(d, pl.lt, backward, st, what);
+    return pl.r == 4 ? by_window<T, 8, 4>(d, pl.lt, backward, st, what) : by_window<T, 8, 8>(d, pl.lt, backward, st, what);
 }
 
 int windows_of(const vk_block_norm_args* a, const Plan& pl)

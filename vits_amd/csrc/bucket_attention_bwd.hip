@@ -3,6 +3,8 @@
 // walks over keys), once for the gradients of the keys and values (a workgroup owns keys and walks
 // over the queries of every head that shares them).  Two walks cost 7 products instead of 5, but every
 // sum has one owner and a fixed order: no atomics, bit-identical from run to run.
+// Measured: 2 x 4095 causal positions, 16 bf16 heads of 128 on 4, 806 us (427 TFLOP/s of the formula's products), bound by
+// matrix and vector instructions of two waves per SIMD that overlap little; 16 x up to 697, 2 fp32 heads of 96, 183 us.
 #include "bucket_attention.hpp"
 #include "api_internal.hpp"
 #include "bucket_attention_host.hpp"

@@ -4,6 +4,10 @@
 // with the running maximum and sum of the softmax.  Scores are computed transposed (rows = keys,
 // columns = queries), so a query is a lane: its maximum and sum are lane-local but for one exchange
 // between the two lane halves, and the probabilities are already the right operand of P V.
+//
+// Bound by the softmax's vector instructions in bf16 (4 x 8191 positions, 8 heads of 64: 728 us, 755 TFLOP/s; per 32 x 32
+// scores 256 cycles of matrix instructions against some 640 of vector instructions), in fp32 by the matrix instruction's
+// rate and unequal lengths (16 x up to 1001 positions, 2 heads of 96: 101 us, 59 TFLOP/s).
 #include "bucket_attention.hpp"
 #include "bucket_attention_narrow.hpp"
 #include "api_internal.hpp"
