@@ -219,7 +219,8 @@ void bucket_attention_narrow_kernel(Dev p)
             }
             if (j0 + NWAVE * TK < end) N::load_keys(kr, kg, p.kc, p.head_dim, j0 + NWAVE * TK, p.keys);
             if (!here) continue;
-            const int side = bias_side(p, j0 - (it.start + i_hi), j0 + TK - 1 - (it.start + i_lo));
+            // by the keys that are there, as for the whole share above: where the table was not staged, no tile takes it
+            const int side = bias_side(p, j0 - (it.start + i_hi), min(j0 + TK, end) - 1 - (it.start + i_lo));
             const float flat = side == BIAS_LEFT ? left : side == BIAS_RIGHT ? right : 0.0f;
             const bool whole = j0 + TK <= end && !(p.causal && j0 + TK - 1 > it.start + i_lo);
             const int stop = p.causal ? min(end, pos + 1) : end;
