@@ -47,3 +47,70 @@ def test_more_queries_than_keys(nk, dtype):
     ref = ref_of(q, k, v, bias, buckets, opts, dout)
     assert_within("lse", lse, ref["lse"])
     assert_within("out", out, ref["out"])
+
+
+# ---- biases that forbid ----------------------------------------------------------------------------
+
+FORBID = [-math.inf, torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min]
+# B, H, Hk, D, Tq, Tk, buckets, causal, nk, nq, start: rows behind nk + max_distance see only the last bucket of the keys behind
+FORBID_CASES = [
+    (1, 2, 1, 64, 300, 300, (16, 40, True), False, [150], None, None),
+    (2, 2, 2, 96, 131, 131, (8, 20, True), False, [90, 131], None, None),
+    (1, 4, 2, 128, 200, 200, (16, 40, True), True, [130], None, None),
+    (9, 16, 4, 128, 257, 257, (16, 40, True), True, None, None, None),
+    (17, 16, 8, 64, 130, 130, (16, 40, True), False, None, None, None),
+]
+FORBID_IDS = [f"B{c[0]}H{c[1]}-{c[2]}D{c[3]}T{c[4]}{'c' if c[7] else ''}" for c in FORBID_CASES]
+
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("value", FORBID, ids=["inf", "lowest32", "lowest16"])
+@pytest.mark.parametrize("which", ["behind", "ahead", "both"])
+@pytest.mark.parametrize("case", FORBID_CASES, ids=FORBID_IDS)
+def test_a_forbidden_bucket(case, which, value, dtype):
+    """The bucket of everything far behind, of everything far ahead, or both, at -inf or at a type's lowest value.
+    A row of which nothing is left is a row without keys.
+
+    The reference takes -800 for the forbidden value: next to any other key of a row the probability is 0 in 64 bits too
+    (logits here are below 30 in magnitude), and the rows that have no other key are behind the reference's query_lengths."""
+    q, k, v, bias, dout, buckets, opts = both(case, dtype)
+    side, far, B, Tq = buckets.num_buckets // 2, buckets.max_distance, case[0], case[4]
+    gone = [b for b, at in ((side - 1, "behind"), (2 * side - 1, "ahead")) if which in (at, "both")]
+    finite = bias.clone()
+    finite[:, gone] = -800.0
+    bias[:, gone] = value
+    first = buckets._side.index(side - 1)                   # the distance at which the last bucket begins
+    nk = case[8] or [case[5]] * B
+    ref_opts = opts | dict(query_lengths=i64([min(Tq, n - 1 + first) if which != "ahead" else Tq for n in nk]))
+    out, lse = bucket_attention(q, k, v, bias, buckets, return_lse=True, **opts)
+    ref = ref_of(q, k, v, finite, buckets, ref_opts, dout)
+    assert_within("lse", lse, ref["lse"])
+    assert_within("out", out, ref["out"])
+    grads = dict(zip(GRADS, bucket_attention_backward(dout, q, k, v, out, lse, bias, buckets, **opts)))
+    for name in GRADS:
+        assert_within(name, grads[name], ref[name])
+    assert not grads["dbias"][:, gone].any()
+
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("value", FORBID, ids=["inf", "lowest32", "lowest16"])
+def test_everything_forbidden(value, dtype):
+    """One head's whole bias forbids: its rows are without keys; the other head is as it was."""
+    for case in ((1, 2, 2, 64, 70, 70, (16, 40, True), False, None, None, None),
+                 (2, 2, 2, 128, 1, 1000, (16, 40, False), True, None, None, [999, 500]),
+                 (9, 16, 16, 128, 257, 257, (16, 40, True), False, None, None, None)):
+        q, k, v, bias, dout, buckets, opts = both(case, dtype)
+        D = case[3]
+        want, want_lse = bucket_attention(q, k, v, bias, buckets, return_lse=True, **opts)
+        want_grads = bucket_attention_backward(dout, q, k, v, want, want_lse, bias, buckets, **opts)
+        bias[0] = value
+        out, lse = bucket_attention(q, k, v, bias, buckets, return_lse=True, **opts)
+        assert not out[:, :D].any() and (lse[:, 0] == -math.inf).all()
+        assert torch.equal(out[:, D:], want[:, D:]) and torch.equal(lse[:, 1:], want_lse[:, 1:])
+        dq, dk, dv, dbias = bucket_attention_backward(dout, q, k, v, out, lse, bias, buckets, **opts)
+        assert not dq[:, :D].any() and not dbias[0].any()
+        assert torch.equal(dq[:, D:], want_grads[0][:, D:]) and torch.equal(dbias[1:], want_grads[3][1:])
+        assert not dk[:, :D].any() and not dv[:, :D].any()
+        assert torch.equal(dk[:, D:], want_grads[1][:, D:]) and torch.equal(dv[:, D:], want_grads[2][:, D:])

@@ -212,9 +212,10 @@ void bucket_dq_kernel(Dev p)
     }
     if (p.bias) {
         if (lse2 < __builtin_inff()) {                      // what the rounding of (bias - lse2) and of lse2 left out
+            // (a bias of -inf: all probabilities there are 0, and -inf - (-inf) is no rounding)
             const float left = tab[0] - lse2, right = tab[2 * p.far_] - lse2;
-            far_left *= 1.0 + (((double)tab[0] - (double)lse2 - (double)left) - off) * (double)LN2;
-            far_right *= 1.0 + (((double)tab[2 * p.far_] - (double)lse2 - (double)right) - off) * (double)LN2;
+            if (left != -__builtin_inff()) far_left *= 1.0 + (((double)tab[0] - (double)lse2 - (double)left) - off) * (double)LN2;
+            if (right != -__builtin_inff()) far_right *= 1.0 + (((double)tab[2 * p.far_] - (double)lse2 - (double)right) - off) * (double)LN2;
         }
         far_left = (double)sgn * far_left + end_left;
         far_right = (double)sgn * far_right + end_right;
