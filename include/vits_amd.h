@@ -365,13 +365,14 @@ int vk_expand_prior(const float* durations, const float* m, const float* logs, f
  * Inference and training, element type `dtype` (VK_DTYPE_F32: exact fp32 matrix instruction;
  * VK_DTYPE_BF16: bf16 matrix inputs, fp32 accumulation and softmax).  Tensors are channel-major views
  * [batch, channels, time] with dense time, as everywhere here; strides count elements.  Batches are
- * padded: `*_lengths[b]` (clamped to the tensor's length; NULL: full) says how far item b goes, and
- * nothing behind it is read.
+ * padded: `*_lengths[b]` (clamped to the tensor's length; NULL: full) says how far item b goes.  What lies behind it,
+ * within the tensor, may be read but enters no result.
  *
  * vk_bucket_attention:  q [B, heads * head_dim, queries], k, v [B, kv_heads * head_dim, keys]; head h reads
  * kv head h / (heads / kv_heads);  pos_i = query_start[b] + i (NULL: i)
  *     s_ij  = scale * q_i . k_j + bias[h, bucket_of[clamp(j - pos_i, +-max_distance) + max_distance]]
- *             over j < key_lengths[b], with `causal` over j <= pos_i
+ *             over j < key_lengths[b], with `causal` over j <= pos_i (keys that this hides from all
+ *                         queries enter no result either: a cache need not be filled up to its length)
  *     lse_i = log sum_j exp(s_ij)          out_i = sum_j exp(s_ij - lse_i) v_j
  * A query without keys, and one at or behind query_lengths[b], gets out = 0 and lse = -inf.
  * bias [heads, buckets] fp32, bucket_of int32 [2 * max_distance + 1] (entries are clamped to the

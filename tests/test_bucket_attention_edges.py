@@ -114,3 +114,29 @@ def test_everything_forbidden(value, dtype):
         assert torch.equal(dq[:, D:], want_grads[0][:, D:]) and torch.equal(dbias[1:], want_grads[3][1:])
         assert not dk[:, :D].any() and not dv[:, :D].any()
         assert torch.equal(dk[:, D:], want_grads[1][:, D:]) and torch.equal(dv[:, D:], want_grads[2][:, D:])
+
+
+# ---- what a pass must not look at ------------------------------------------------------------------
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("val", [math.nan, math.inf])
+@pytest.mark.parametrize("case", [
+    (2, 8, 2, 64, 8, 500, (32, 128, False), True, None, [3, 8], [100, 77]),        # a padded chunk of new tokens, a cache not yet full
+    (1, 2, 2, 96, 40, 200, (32, 128, False), True, None, [21], [90]),
+    (2, 16, 4, 128, 150, 400, (32, 128, False), True, None, [101, 0], [30, 5]),
+    (1, 4, 1, 64, 1, 1000, (32, 128, False), True, None, None, [637]),
+], ids=lambda c: f"B{c[0]}H{c[1]}-{c[2]}D{c[3]}T{c[4]}-{c[5]}")
+def test_keys_that_causal_hides_from_every_query(case, val, dtype):
+    """A causal cache without key_lengths: what lies behind the last query's position may hold anything."""
+    q, k, v, bias, dout, buckets, opts = both(case, dtype)
+    nq = case[9] or [case[4]] * case[0]
+    seen = i64([s + n if n else 0 for s, n in zip(case[10], nq)])
+    hidden = torch.arange(case[5], device="cuda") >= seen.view(-1, 1, 1)
+    out, lse = bucket_attention(q, k, v, bias, buckets, return_lse=True, **opts)
+    grads = bucket_attention_backward(dout, q, k, v, out, lse, bias, buckets, **opts)
+    k2, v2 = k.masked_fill(hidden, val), v.masked_fill(hidden, val)
+    out2, lse2 = bucket_attention(q, k2, v2, bias, buckets, return_lse=True, **opts)
+    assert torch.equal(out2, out) and torch.equal(lse2, lse)
+    for a, b in zip(bucket_attention_backward(dout, q, k2, v2, out, lse, bias, buckets, **opts), grads):
+        assert torch.equal(a, b)

@@ -178,8 +178,9 @@ def bucket_attention(q, k, v, bias=None, buckets: RelativeBuckets | None = None,
     bias: float32 ``[heads, buckets.num_buckets]``, or None (no position bias); -inf or a type's lowest value (below -2.35e38)
     forbids a bucket, and a query that may see nothing else is one without a key.  key_lengths, query_lengths, query_start:
     int64 ``[B]`` on the device, or None.  scale: 1 / sqrt(D) unless given, positive.  Queries without a key and those at or behind
-    query_lengths[b] come out as zero; nothing behind a length is read, so padding may hold anything.  Serving a new
-    token over a cache: Tq = 1, query_start = key_lengths - 1; the cache may be a view of a larger buffer.
+    query_lengths[b] come out as zero.  What lies behind a length enters no result, nor do keys that ``causal`` hides from all
+    of an item's queries: padding may hold anything.  Serving a new token over a cache: Tq = 1, query_start = key_lengths - 1;
+    the cache may be a view of a larger buffer.
 
     Returns out ``[B, heads * D, Tq]``, with ``return_lse`` also the log-sum-exp of the logits ``[B, heads, Tq]`` (-inf
     where there is no key), which ``bucket_attention_backward`` takes and which carries no gradient."""

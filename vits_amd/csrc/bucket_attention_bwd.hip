@@ -320,7 +320,9 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
             dot_channels<DP, PT>(s, qim, c0, kf);
             if constexpr (DK) dot_channels<DP, PT>(dp, dim, c0, vf);
             const float flat = bias_flat(tab, p, side);
-            if (side != BIAS_NEAR && !(p.causal && hi > 0)) {
+            // with `causal`, a key that only queries behind their length would see may hold anything: they are masked too
+            const int stop = it.nq - is;
+            if (side != BIAS_NEAR && !(p.causal && (hi > 0 || stop < 32))) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], p.c, flat - st[c0 + acc_row(r, h)]));
             } else {
@@ -329,7 +331,10 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
                     const int row = acc_row(r, h), off = j - (pos0 + row);
                     const float bias = side == BIAS_NEAR ? tab[clampi(off, -p.far_, p.far_) + p.far_] : flat;
                     s[r] = exp2_hw(fmaf(s[r], p.c, bias - st[c0 + row]));
-                    if (p.causal && off > 0) s[r] = 0.0f;
+                    if (p.causal && (off > 0 || row >= stop)) {
+                        s[r] = 0.0f;
+                        if constexpr (DK) dp[r] = 0.0f;
+                    }
                 }
             }
             if constexpr (DV) dot_positions<DP, PT>(dv, dim, c0, s);

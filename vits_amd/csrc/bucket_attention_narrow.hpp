@@ -154,7 +154,7 @@ void bucket_attention_narrow_kernel(Dev p)
     const int i_lo = g0 == g1 ? r0 - g0 * p.queries : 0, i_hi = g0 == g1 ? last - g0 * p.queries : p.queries - 1;
 
     int end = it.nk;
-    if (p.causal) end = clampi(it.start + i_hi + 1, 0, end);
+    if (p.causal) end = clampi(it.start + min(i_hi, it.nq - 1) + 1, 0, end);      // behind it may lie anything
     if (i_lo >= it.nq) end = 0;
     const int first = split * p.per_split * TK;
     end = min(end, first + p.per_split * TK);
