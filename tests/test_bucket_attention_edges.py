@@ -140,3 +140,21 @@ def test_keys_that_causal_hides_from_every_query(case, val, dtype):
     assert torch.equal(out2, out) and torch.equal(lse2, lse)
     for a, b in zip(bucket_attention_backward(dout, q, k2, v2, out, lse, bias, buckets, **opts), grads):
         assert torch.equal(a, b)
+
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("D", [40, 64, 33, 5])
+@pytest.mark.parametrize("Tq,Tk", [(1, 700), (43, 43), (200, 200)])
+def test_an_infinite_key(D, Tq, Tk, dtype):
+    """A last key with an infinity in its last channel, which every query turns into -inf: the same as without that key,
+    whatever the head's width."""
+    b = RelativeBuckets(8, 20)
+    q, k, v, bias, _ = inputs(dtype, 2, 2, 2, D, Tq, Tk, b)
+    q.view(2, 2, D, Tq)[:, :, -1] = -q.view(2, 2, D, Tq)[:, :, -1].abs() - 0.1
+    k.view(2, 2, D, Tk)[:, :, -1, -1] = math.inf
+    out, lse = bucket_attention(q, k, v, bias, b, heads=2, return_lse=True)
+    ref = ref_of(q, k, v, bias, b, dict(heads=2, kv_heads=2, key_lengths=i64([Tk - 1] * 2), query_lengths=None, query_start=None,
+                                        causal=False))
+    assert_within("out", out, ref["out"])
+    assert_within("lse", lse, ref["lse"])

@@ -42,9 +42,13 @@ struct Narrow {
             for (int n = 0; n < NK; ++n) __builtin_memcpy(&k[n], p + (int64_t)krow(n, 0) * cstride * (int64_t)sizeof(T) + lane, 16);
             return;
         }
-        // channels that are not there: any others, the queries are zero for them
+        // channels that are not there: zero, for another channel's infinity would make a NaN of the queries' zero
 #pragma unroll
-        for (int n = 0; n < NK; ++n) __builtin_memcpy(&k[n], base + (int64_t)min(krow(n, q4), d_real - 1) * cstride + col, 16);
+        for (int n = 0; n < NK; ++n) {
+            const int d = krow(n, q4);
+            __builtin_memcpy(&k[n], base + (int64_t)min(d, d_real - 1) * cstride + col, 16);
+            k[n] = d < d_real ? k[n] : u32x4{0u, 0u, 0u, 0u};
+        }
     }
     // Values: load (blk, r) of a lane is channel 16 blk + lane % 16, positions base + 4 E r + E (lane / 16); zero at and
     // behind `limit`, whatever lies there.
