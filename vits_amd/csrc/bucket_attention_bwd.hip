@@ -105,7 +105,7 @@ void bucket_dq_kernel(Dev p)
     double off = 0.0;
     if (valid) {
         const float v = p.lse_in[row];
-        if (v != -__builtin_inff()) {                       // without keys all probabilities are 0
+        if (v != -__builtin_inff()) {                             // without keys all probabilities are 0
             lse2 = v * LOG2E;
             off = (double)v * 1.4426950408889634 - (double)lse2;
         }
@@ -320,18 +320,24 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
             dot_channels<DP, PT>(s, qim, c0, kf);
             if constexpr (DK) dot_channels<DP, PT>(dp, dim, c0, vf);
             const float flat = bias_flat(tab, p, side);
-            // with `causal`, a key that only queries behind their length would see may hold anything: they are masked too
-            const int stop = it.nq - is;
-            if (side != BIAS_NEAR && !(p.causal && (hi > 0 || stop < 32))) {
+            if (side != BIAS_NEAR) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = exp2_hw(fmaf(s[r], p.c, flat - st[c0 + acc_row(r, h)]));
             } else {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int row = acc_row(r, h), off = j - (pos0 + row);
-                    const float bias = side == BIAS_NEAR ? tab[clampi(off, -p.far_, p.far_) + p.far_] : flat;
+                    const int row = acc_row(r, h);
+                    const float bias = tab[clampi(j - (pos0 + row), -p.far_, p.far_) + p.far_];
                     s[r] = exp2_hw(fmaf(s[r], p.c, bias - st[c0 + row]));
-                    if (p.causal && (off > 0 || row >= stop)) {
+                }
+            }
+            // queries behind their length are masked too: a key that only they would see may hold anything
+            const int stop = it.nq - is;
+            if (p.causal && (hi > 0 || stop < 32)) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int row = acc_row(r, h);
+                    if (j > pos0 + row || row >= stop) {
                         s[r] = 0.0f;
                         if constexpr (DK) dp[r] = 0.0f;
                     }

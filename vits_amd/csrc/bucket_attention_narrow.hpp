@@ -42,12 +42,19 @@ struct Narrow {
             for (int n = 0; n < NK; ++n) __builtin_memcpy(&k[n], p + (int64_t)krow(n, 0) * cstride * (int64_t)sizeof(T) + lane, 16);
             return;
         }
-        // channels that are not there: zero, for another channel's infinity would make a NaN of the queries' zero
+        // Channels that are not there, among the last 32, are zero: another channel's infinity would make a NaN of the
+        // queries' zero.
+        int real = d_real;
+        asm volatile("" : "+s"(real));                              // masks made where they are used, not kept over the loop
 #pragma unroll
         for (int n = 0; n < NK; ++n) {
             const int d = krow(n, q4);
-            __builtin_memcpy(&k[n], base + (int64_t)min(d, d_real - 1) * cstride + col, 16);
-            k[n] = d < d_real ? k[n] : u32x4{0u, 0u, 0u, 0u};
+            if (krow(n, 0) < DP - 32) {
+                __builtin_memcpy(&k[n], base + (int64_t)d * cstride + col, 16);
+            } else {
+                __builtin_memcpy(&k[n], base + (int64_t)min(d, real - 1) * cstride + col, 16);
+                k[n] &= (unsigned)((d - real) >> 31);
+            }
         }
     }
     // Values: load (blk, r) of a lane is channel 16 blk + lane % 16, positions base + 4 E r + E (lane / 16); zero at and
