@@ -385,7 +385,8 @@ int vk_expand_prior(const float* durations, const float* m, const float* logs, f
  *     p = exp(s - lse), ds_ij = p_ij (dout_i . v_j - dout_i . out_i)
  *     dq = scale ds k, dk = scale ds^T q, dv = p^T dout (summed over the heads that share a kv head),
  *     dbias[h, c] = sum of ds_ij of head h over all pairs of bucket c (fp32)
- * All four are written whole (zero where nothing contributes), in a fixed order of summation.        */
+ * All four are written whole (zero where nothing contributes), in a fixed order of summation.  A row with lse < -2^20 (all
+ * its keys have a bias that low; fp32 does not hold what exp(s - lse) needs there) passes no gradient back.       */
 #define VK_DTYPE_F32   0
 #define VK_DTYPE_BF16  1
 #define VK_BUCKET_MAX_HEAD_DIM 128

@@ -116,6 +116,37 @@ def test_everything_forbidden(value, dtype):
         assert torch.equal(dk[:, D:], want_grads[1][:, D:]) and torch.equal(dv[:, D:], want_grads[2][:, D:])
 
 
+# ---- biases that are finite, but so low that an fp32 logit holds nothing else ------------------------
+
+@gpu
+@TYPES
+@pytest.mark.parametrize("value", [-1e9, -1e10, -1e30])
+@pytest.mark.parametrize("case", FORBID_CASES[:1] + FORBID_CASES[2:4], ids=FORBID_IDS[:1] + FORBID_IDS[2:4])
+def test_a_very_low_bias_under_large_logits(case, value, dtype):
+    """Everything far behind at a very low finite value, logits up to some 200: the first keys of a row are all far behind,
+    so the running maximum starts there.  Rows with no other key come out finite, and pass no gradient back: their lse, in
+    fp32, does not hold what their probabilities need.
+
+    The reference takes -4000, as above."""
+    q, k, v, bias, dout, buckets, opts = both(case, dtype)
+    q = (q.float() * 50).to(dtype)
+    side, B, Tq = buckets.num_buckets // 2, case[0], case[4]
+    finite = bias.clone()
+    finite[:, side - 1] = -4000.0
+    bias[:, side - 1] = value
+    first = buckets._side.index(side - 1)
+    nk = case[8] or [case[5]] * B
+    cut = i64([min(Tq, n - 1 + first) for n in nk])
+    live = torch.arange(Tq, device="cuda") < cut.view(-1, 1, 1)
+    out, lse = bucket_attention(q, k, v, bias, buckets, return_lse=True, **opts)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    ref = ref_of(q, k, v, finite, buckets, opts | dict(query_lengths=cut), dout)
+    assert_within("lse", torch.where(live, lse, -math.inf), ref["lse"])
+    assert_within("out", torch.where(live, out, 0), ref["out"])
+    for name, g in zip(GRADS, bucket_attention_backward(dout, q, k, v, out, lse, bias, buckets, **opts)):
+        assert_within(name, g, ref[name])
+
+
 # ---- what a pass must not look at ------------------------------------------------------------------
 
 @gpu

@@ -201,7 +201,8 @@ def bucket_attention_backward(dout, q, k, v, out, lse, bias=None, buckets: Relat
     """Gradients (dq, dk, dv, dbias) of ``bucket_attention`` for the gradient ``dout`` of its output, from what it took
     and gave (``out``, ``lse``); dbias is None without a bias.  dout and out may have any strides (without a dense time
     axis they are copied).  Every sum has a fixed order: the same inputs give the
-    same bits.  Padding gets zero gradients."""
+    same bits.  Padding gets zero gradients, and so does a query all of whose keys have a bias so low that lse < -2^20: fp32
+    does not hold its probabilities there."""
     kv_heads, scale, table = _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, query_start, scale)
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:

@@ -32,6 +32,10 @@ struct Shape {
 
 __host__ __device__ inline int64_t kv_elements(const Dev& p) { return (int64_t)p.batch * (p.heads / p.group) * p.head_dim * p.keys; }
 
+// A row whose log-sum-exp is below this (all its keys have a bias that low) passes no gradient back: fp32 does not hold
+// what its probabilities need (a step is 2^-3 here and grows), and exp(s - lse) would grow out of bounds.
+constexpr float LSE_LEAST = -0x1p20f;
+
 constexpr int DGP = 33;         // pitch of a wave's 32 x 32 block of logit gradients
 
 // dq_i = scale * sum_j ds_ij k_j, and the sums of ds over the diagonals j - pos_i = const (the bias
@@ -105,7 +109,7 @@ void bucket_dq_kernel(Dev p)
     double off = 0.0;
     if (valid) {
         const float v = p.lse_in[row];
-        if (v != -__builtin_inff()) {                             // without keys all probabilities are 0
+        if (!(v < LSE_LEAST)) {                             // without keys all probabilities are 0
             lse2 = v * LOG2E;
             off = (double)v * 1.4426950408889634 - (double)lse2;
         }
@@ -304,7 +308,7 @@ __device__ __forceinline__ void key_side(const Dev& p, int id, unsigned char* ld
         __syncthreads();
         qt.store(qim);
         dt.store(dim);
-        if (threadIdx.x < KT) st[threadIdx.x] = stat == -__builtin_inff() ? __builtin_inff() : stat * LOG2E;    // no keys: all probabilities 0
+        if (threadIdx.x < KT) st[threadIdx.x] = stat < LSE_LEAST ? __builtin_inff() : stat * LOG2E;    // no keys: all probabilities 0
         else if (threadIdx.x < 2 * KT) st[threadIdx.x] = -stat;
         if (tile == 0 || step == first) stage_bias(tab, p, kvh * p.group + g);
         __syncthreads();

@@ -17,6 +17,15 @@ namespace {
 using namespace vkba;
 
 constexpr int FWD_TILE = 64;    // keys of a staged tile
+// A bias that a whole block shares enters the exponents as flat - maximum, exactly, while the maximum is rounded with the
+// bias in it: they differ by up to half a step of the bias, 16 just below FLAT_MAX, and an exponent is that much too large.
+// Ends of the table (bits: left, right) that are larger, but finite, are looked up like near ones.
+constexpr float FLAT_MAX = 0x1p29f;
+__device__ __forceinline__ int steep_ends(const float* tab, const Dev& p)
+{
+    auto steep = [](float x) { return fabsf(x) >= FLAT_MAX && fabsf(x) < __builtin_inff(); };
+    return __builtin_amdgcn_readfirstlane((steep(tab[0]) ? 1 << BIAS_LEFT : 0) | (steep(tab[2 * p.far_]) ? 1 << BIAS_RIGHT : 0));
+}
 
 // KW = 2: half of the waves take the first, half the second 32 keys of every tile (64 queries per workgroup
 // instead of 128), each with a maximum, sum and output of its own, joined through LDS at the end.  The staging of
@@ -81,6 +90,7 @@ void bucket_attention_kernel(Dev p)
 
     const float c = p.c;
     const int pos0 = it.start + q0, pos = pos0 + (l & 31);
+    const int steep = p.bias && first < end ? steep_ends(tab, p) : 0;
     for (int j0 = first; j0 < end; j0 += KT) {
         if constexpr (!AHEAD) {
             kt.load(kg, p.kc, p.head_dim, j0, end);
@@ -107,7 +117,8 @@ void bucket_attention_kernel(Dev p)
             }
             float mul = c, flat = 0.0f;                                         // logit = mul * s + flat
             const int lo = js - (pos0 + 31), hi = js + 32 * SP - 1 - pos0;
-            const int side = bias_side(p, lo, hi);
+            int side = bias_side(p, lo, hi);
+            if (steep >> side & 1) side = BIAS_NEAR;
             if (side == BIAS_NEAR) {
                 mul = 1.0f;
 #pragma unroll
