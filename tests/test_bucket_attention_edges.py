@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_bucket_attention import _args, assert_within, both, i64, inputs, ref_of
-from vits_amd import native
+from vits_amd import attention, native
 from vits_amd.attention import RelativeBuckets, bucket_attention, bucket_attention_backward
 
 gpu = pytest.mark.gpu
@@ -189,3 +189,19 @@ def test_an_infinite_key(D, Tq, Tk, dtype):
                                         causal=False))
     assert_within("out", out, ref["out"])
     assert_within("lse", lse, ref["lse"])
+
+
+# ---- state, and other kinds of differentiation -------------------------------------------------------
+
+@gpu
+def test_a_validation_pass_before_training():
+    """The bucket table is first used under inference_mode, then by a call that autograd records."""
+    case = (1, 2, 2, 32, 21, 21, (8, 16, True), False, None, None, None)
+    q, k, v, bias, dout, buckets, opts = both(case, torch.float32)
+    with torch.inference_mode():
+        want = bucket_attention(q, k, v, bias, buckets, **opts)
+    with torch.enable_grad():
+        leaves = [t.clone().requires_grad_() for t in (q, k, v, bias)]
+        out = bucket_attention(*leaves, buckets, **opts)
+        out.backward(dout)
+    assert torch.equal(out, want) and all(t.grad is not None for t in leaves)

@@ -65,8 +65,9 @@ class RelativeBuckets:
             key = native._device_index(device)
             if torch.cuda.is_current_stream_capturing():
                 raise native.NativeError("call RelativeBuckets.table(device) before the capture")
-            t = torch.tensor([self.bucket_of(o) for o in range(-self.max_distance, self.max_distance + 1)],
-                             dtype=torch.int32).to(torch.device("cuda", key))
+            with torch.inference_mode(False):               # a table first used there has to serve autograd too
+                t = torch.tensor([self.bucket_of(o) for o in range(-self.max_distance, self.max_distance + 1)],
+                                 dtype=torch.int32).to(torch.device("cuda", key))
             self._tables[key] = self._tables[device.index] = t
         return t
 
