@@ -205,3 +205,17 @@ def test_a_validation_pass_before_training():
         out = bucket_attention(*leaves, buckets, **opts)
         out.backward(dout)
     assert torch.equal(out, want) and all(t.grad is not None for t in leaves)
+
+
+def test_the_table_of_an_unnamed_device_is_the_current_ones(monkeypatch):
+    b = RelativeBuckets(8, 18)
+    monkeypatch.setattr(attention, "_TABLES", {}, raising=False)
+    current = [0]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, device, *a: (self, device))
+    first = b.table("cuda")
+    current[0] = 1
+    second = b.table("cuda")
+    assert first[1] == torch.device("cuda", 0) and second[1] == torch.device("cuda", 1)
+    assert b.table(torch.device("cuda", 1)) is second and b.table("cuda:0") is first

@@ -59,16 +59,15 @@ class RelativeBuckets:
     def table(self, device) -> torch.Tensor:
         """int32 [2 * max_distance + 1] on ``device``: the bucket of every offset from -max_distance up.
         Made once per device."""
-        device = torch.device(device)
-        t = self._tables.get(device.index)
+        index = native._device_index(device)                # of "cuda" alone: the current device's, whichever that is
+        t = self._tables.get(index)
         if t is None:
-            key = native._device_index(device)
             if torch.cuda.is_current_stream_capturing():
                 raise native.NativeError("call RelativeBuckets.table(device) before the capture")
             with torch.inference_mode(False):               # a table first used there has to serve autograd too
                 t = torch.tensor([self.bucket_of(o) for o in range(-self.max_distance, self.max_distance + 1)],
-                                 dtype=torch.int32).to(torch.device("cuda", key))
-            self._tables[key] = self._tables[device.index] = t
+                                 dtype=torch.int32).to(torch.device("cuda", index))
+            self._tables[index] = t
         return t
 
 
