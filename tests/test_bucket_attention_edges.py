@@ -219,3 +219,24 @@ def test_the_table_of_an_unnamed_device_is_the_current_ones(monkeypatch):
     second = b.table("cuda")
     assert first[1] == torch.device("cuda", 0) and second[1] == torch.device("cuda", 1)
     assert b.table(torch.device("cuda", 1)) is second and b.table("cuda:0") is first
+
+
+@gpu
+def test_a_graph_outlives_the_buckets_it_was_captured_with():
+    """The table belongs to the buckets' numbers, not to the object: it is not given back while a graph still reads it."""
+    b = RelativeBuckets(8, 22)
+    q, k, v, bias, _ = inputs(torch.float32, 1, 2, 2, 32, 50, 50, b)
+    want = bucket_attention(q, k, v, bias, b, heads=2)
+    size = b.table("cuda").numel()
+    gr = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(gr):
+        out = bucket_attention(q, k, v, bias, b, heads=2)
+    del b
+    others = [torch.full((size,), 7, device="cuda", dtype=torch.int32) for _ in range(64)]      # would take its place
+    for _ in range(3):
+        out.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    del others

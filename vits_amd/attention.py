@@ -22,6 +22,11 @@ import torch
 from . import native
 
 
+# Bucket tables by device and contents, a few KiB each, kept for good: a graph, or a call still running on another
+# stream, may read one after the RelativeBuckets it was made for is gone.
+_TABLES = {}
+
+
 class RelativeBuckets:
     """Buckets of the offset key - query.  Half of the buckets are for keys ahead of the query, half for
     keys at or behind it (``bidirectional=False``: all for keys at or behind it, those ahead share bucket
@@ -58,15 +63,18 @@ class RelativeBuckets:
 
     def table(self, device) -> torch.Tensor:
         """int32 [2 * max_distance + 1] on ``device``: the bucket of every offset from -max_distance up.
-        Made once per device."""
+        Made once per device, and there for good."""
         index = native._device_index(device)                # of "cuda" alone: the current device's, whichever that is
         t = self._tables.get(index)
         if t is None:
+            # not even where another object has made this table: whether a call can be captured does not hang on that
             if torch.cuda.is_current_stream_capturing():
                 raise native.NativeError("call RelativeBuckets.table(device) before the capture")
-            with torch.inference_mode(False):               # a table first used there has to serve autograd too
-                t = torch.tensor([self.bucket_of(o) for o in range(-self.max_distance, self.max_distance + 1)],
-                                 dtype=torch.int32).to(torch.device("cuda", index))
+            of = tuple(self.bucket_of(o) for o in range(-self.max_distance, self.max_distance + 1))
+            t = _TABLES.get((index, of))
+            if t is None:
+                with torch.inference_mode(False):           # a table first used there has to serve autograd too
+                    t = _TABLES[index, of] = torch.tensor(of, dtype=torch.int32).to(torch.device("cuda", index))
             self._tables[index] = t
         return t
 
