@@ -1,0 +1,37 @@
+"""The norms around a block at the edges of their definition.  The 64-bit reference and the derived bounds are those of
+test_block_norm.py."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from test_block_norm import _args, assert_within, grads_dict, inputs, reference
+from vits_amd import native
+from vits_amd.block_norm import block_norm, block_norm_backward
+
+gpu = pytest.mark.gpu
+TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+
+
+@gpu
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    d, dh, dn = inputs(torch.float32, 1, 16, 8)
+    h, n = block_norm(**d)
+    keep = {k: v for k, v in d.items() if k not in ("x", "y")}
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for name in ("x", "y", "gate", "scale"):
+            with pytest.raises(native.NativeError, match="forward"):
+                block_norm(**(d | {name: dual(d[name])}))
+        for name in ("post", "pre"):
+            for i in range(2):
+                pair = list(d[name])
+                pair[i] = dual(pair[i])
+                with pytest.raises(native.NativeError, match="forward"):
+                    block_norm(**(d | {name: tuple(pair)}))
+        for args in ((dual(dh), dn, h, d["y"]), (dh, dual(dn), h, d["y"]), (dh, dn, dual(h), d["y"]), (dh, dn, h, dual(d["y"]))):
+            with pytest.raises(native.NativeError, match="forward"):
+                block_norm_backward(*args, **keep)
+        assert torch.equal(block_norm(**d)[0], h)

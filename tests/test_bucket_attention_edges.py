@@ -222,6 +222,25 @@ def test_the_table_of_an_unnamed_device_is_the_current_ones(monkeypatch):
 
 
 @gpu
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    b = RelativeBuckets(8, 20)
+    q, k, v, bias, dout = inputs(torch.float32, 1, 1, 1, 32, 16, 16, b)
+    out, lse = bucket_attention(q, k, v, bias, b, heads=1, return_lse=True)
+    with fwd.dual_level():
+        for n in range(4):
+            args = [q, k, v, bias]
+            args[n] = fwd.make_dual(args[n], torch.ones_like(args[n]))
+            with pytest.raises(native.NativeError, match="forward"):
+                bucket_attention(*args, b, heads=1)
+            with pytest.raises(native.NativeError, match="forward"):
+                bucket_attention_backward(dout, *args[:3], out, lse, args[3], b, heads=1)
+        with pytest.raises(native.NativeError, match="forward"):
+            bucket_attention_backward(fwd.make_dual(dout, dout), q, k, v, out, lse, bias, b, heads=1)
+        assert torch.equal(bucket_attention(q, k, v, bias, b, heads=1), out)
+
+
+@gpu
 def test_a_graph_outlives_the_buckets_it_was_captured_with():
     """The table belongs to the buckets' numbers, not to the object: it is not given back while a graph still reads it."""
     b = RelativeBuckets(8, 22)

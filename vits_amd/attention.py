@@ -10,7 +10,7 @@ with dense time (slices of a fused projection go in as they are), fp32 or bf16.
     buckets = RelativeBuckets(32, 128)
     out = bucket_attention(q, k, v, bias, buckets, heads=8, key_lengths=n, query_lengths=n)
 
-``bucket_attention`` records itself for autograd.  Recording while a stream is captured into a HIP graph
+``bucket_attention`` records itself for autograd (reverse mode; forward-mode tangents are refused).  Recording while a stream is captured into a HIP graph
 is refused: autograd's own accumulation nodes for leaves that an earlier eager pass has touched would be
 captured with the stream of that pass.  A training step that is captured calls ``bucket_attention`` under
 ``torch.no_grad()`` (with ``return_lse``) and ``bucket_attention_backward``.
@@ -18,6 +18,7 @@ captured with the stream of that pass.  A training step that is captured calls `
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 
@@ -156,6 +157,13 @@ def _refuse_capture(what):
                                  "and its *_backward function")
 
 
+def _refuse_forward_mode(what, *tensors):
+    """Dual tensors of forward-mode differentiation do not say ``requires_grad``: without this, their tangents got lost."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 \
+            and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise native.NativeError(f"{what} has no forward-mode derivative")
+
+
 class _BucketAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, table, heads, kv_heads, key_lengths, query_lengths, query_start, causal, scale):
@@ -193,6 +201,7 @@ def bucket_attention(q, k, v, bias=None, buckets: RelativeBuckets | None = None,
     Returns out ``[B, heads * D, Tq]``, with ``return_lse`` also the log-sum-exp of the logits ``[B, heads, Tq]`` (-inf
     where there is no key), which ``bucket_attention_backward`` takes and which carries no gradient."""
     kv_heads, scale, table = _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, query_start, scale)
+    _refuse_forward_mode("bucket_attention", q, k, v, bias)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (bias is not None and bias.requires_grad)):
         _refuse_capture("bucket_attention")
@@ -212,6 +221,7 @@ def bucket_attention_backward(dout, q, k, v, out, lse, bias=None, buckets: Relat
     same bits.  Padding gets zero gradients, and so does a query all of whose keys have a bias so low that lse < -2^20: fp32
     does not hold its probabilities there."""
     kv_heads, scale, table = _check(q, k, v, bias, buckets, heads, kv_heads, key_lengths, query_lengths, query_start, scale)
+    _refuse_forward_mode("bucket_attention_backward", dout, q, k, v, out, lse, bias)
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"{name} must be {tuple(q.shape)} of {q.dtype} on {q.device}")

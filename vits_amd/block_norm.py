@@ -8,7 +8,7 @@ backward pass, on the HIP kernels of csrc/block_norm.hip.
 It stands next to ``native.channel_norm`` (LayerNorm over 192 channels, fp32, forward only).  Tensors are channel-major
 ``[batch, channels, time]`` views with dense time, fp32 or bf16; the norms run over the channels.
 
-``block_norm`` records itself for autograd; recording while a stream is captured into a HIP graph is refused (see
+``block_norm`` records itself for autograd (reverse mode; forward-mode tangents are refused); recording while a stream is captured into a HIP graph is refused (see
 ``vits_amd.attention``): capture ``block_norm`` under ``torch.no_grad()`` and ``block_norm_backward``.
 """
 from __future__ import annotations
@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from . import native
-from .attention import _lengths, _refuse_capture, _view3
+from .attention import _lengths, _refuse_capture, _refuse_forward_mode, _view3
 
 _NORMS = {"layer": native.NORM_LAYER, "rms": native.NORM_RMS}
 
@@ -136,6 +136,7 @@ def block_norm(x, y=None, *, post=None, gate=None, scale=None, pre=None, norm: s
     _check(x, y, gate, scale, post, pre, norm, eps, lengths)
     w_post, b_post = post or (None, None)
     w_pre, b_pre = pre or (None, None)
+    _refuse_forward_mode("block_norm", x, y, gate, scale, w_post, b_post, w_pre, b_pre)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (x, y, gate, scale, w_post, b_post, w_pre, b_pre)):
         _refuse_capture("block_norm")
@@ -155,6 +156,7 @@ def block_norm_backward(dh, dn, h, y=None, *, post=None, gate=None, scale=None, 
     if dn is not None and pre is None:
         raise ValueError("dn needs pre")
     _check(h, y, gate, scale, post, pre, norm, eps, lengths)
+    _refuse_forward_mode("block_norm_backward", dh, dn, h, y, gate, scale, *(post or ()), *(pre or ()))
     for name, t in (("dh", dh), ("dn", dn)):
         if t is not None and (tuple(t.shape) != tuple(h.shape) or t.dtype != h.dtype or t.device != h.device):
             raise ValueError(f"{name} must be {tuple(h.shape)} of {h.dtype} on {h.device}")
