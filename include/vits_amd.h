@@ -423,7 +423,8 @@ int vk_bucket_attention_backward(const vk_bucket_attention_args* a, void* stream
  * N over the channels of each column (b, t): VK_NORM_LAYER (v - mean) / sqrt(var + eps), VK_NORM_RMS
  * v / sqrt(mean of squares + eps); statistics and parameters fp32, x, y, gate, h, n of type `dtype`.  n is taken of h
  * before h is rounded for storage.  gate: [B, C, T], or with gate_per_item one value per item and channel
- * (strides gate_bstride, gate_cstride).  Columns at or behind lengths[b] (NULL: none) are not read and written as 0.
+ * (strides gate_bstride, gate_cstride).  Columns at or behind lengths[b] (NULL: none) enter no result and are written
+ * as 0; the gate of an item without columns enters none either.
  * h or n may be NULL (not wanted).  channels <= VK_BLOCK_NORM_MAX_CHANNELS, eps > 0; an item's view spans less than 2^30
  * elements.  Outputs must not overlap inputs.
  *

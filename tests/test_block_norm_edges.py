@@ -15,6 +15,29 @@ TYPES = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["
 
 
 @gpu
+@TYPES
+@pytest.mark.parametrize("norm", ["layer", "rms"])
+@pytest.mark.parametrize("val", [math.nan, math.inf])
+def test_the_gate_of_an_empty_item_may_hold_anything(val, norm, dtype):
+    """A gate per item that was, say, a mean over no columns: it is not part of any sum."""
+    lengths = torch.tensor([37, 0, 21], device="cuda")
+    d, dh, dn = inputs(dtype, 3, 96, 37, gate="item")
+    h, n = block_norm(**d, norm=norm, lengths=lengths)
+    keep = {k: v for k, v in d.items() if k not in ("x", "y")}
+    want = grads_dict(block_norm_backward(dh, dn, h, d["y"], **keep, norm=norm, lengths=lengths))
+    ref = reference(None, d["y"], d["gate"], d["scale"], d["post"], d["pre"], norm, 1e-5, lengths, dh, dn, h)
+    d["gate"] = d["gate"].clone()
+    d["gate"][1] = val
+    keep["gate"] = d["gate"]
+    h2, n2 = block_norm(**d, norm=norm, lengths=lengths)
+    assert torch.equal(h2, h) and torch.equal(n2, n)
+    got = grads_dict(block_norm_backward(dh, dn, h, d["y"], **keep, norm=norm, lengths=lengths))
+    for name in want:
+        assert_within(name, got[name], ref[name])
+        assert torch.equal(got[name], want[name]), name
+
+
+@gpu
 def test_forward_mode_is_refused():
     import torch.autograd.forward_ad as fwd
     d, dh, dn = inputs(torch.float32, 1, 16, 8)

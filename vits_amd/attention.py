@@ -10,10 +10,10 @@ with dense time (slices of a fused projection go in as they are), fp32 or bf16.
     buckets = RelativeBuckets(32, 128)
     out = bucket_attention(q, k, v, bias, buckets, heads=8, key_lengths=n, query_lengths=n)
 
-``bucket_attention`` records itself for autograd (reverse mode; forward-mode tangents are refused).  Recording while a stream is captured into a HIP graph
-is refused: autograd's own accumulation nodes for leaves that an earlier eager pass has touched would be
-captured with the stream of that pass.  A training step that is captured calls ``bucket_attention`` under
-``torch.no_grad()`` (with ``return_lse``) and ``bucket_attention_backward``.
+``bucket_attention`` records itself for autograd (reverse mode; forward-mode tangents are refused).  Recording
+while a stream is captured into a HIP graph is refused: autograd's own accumulation nodes for leaves that an
+earlier eager pass has touched would be captured with the stream of that pass.  A training step that is captured
+calls ``bucket_attention`` under ``torch.no_grad()`` (with ``return_lse``) and ``bucket_attention_backward``.
 """
 from __future__ import annotations
 

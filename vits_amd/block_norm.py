@@ -8,8 +8,9 @@ backward pass, on the HIP kernels of csrc/block_norm.hip.
 It stands next to ``native.channel_norm`` (LayerNorm over 192 channels, fp32, forward only).  Tensors are channel-major
 ``[batch, channels, time]`` views with dense time, fp32 or bf16; the norms run over the channels.
 
-``block_norm`` records itself for autograd (reverse mode; forward-mode tangents are refused); recording while a stream is captured into a HIP graph is refused (see
-``vits_amd.attention``): capture ``block_norm`` under ``torch.no_grad()`` and ``block_norm_backward``.
+``block_norm`` records itself for autograd (reverse mode; forward-mode tangents are refused); recording while a stream
+is captured into a HIP graph is refused (see ``vits_amd.attention``): capture ``block_norm`` under ``torch.no_grad()`` and
+``block_norm_backward``.
 """
 from __future__ import annotations
 
@@ -132,7 +133,8 @@ def block_norm(x, y=None, *, post=None, gate=None, scale=None, pre=None, norm: s
     x, y: ``[B, C, T]``.  post, pre: (weight, bias) of the norm after the block and of the one before the next, bias may be
     None; without ``post`` y is taken as it is, without ``pre`` n is None.  gate: ``[B, C, T]`` or ``[B, C, 1]`` (one value per
     item and channel); scale: ``[C]``.  Parameters are float32.  Without y there is only the norm of x: h is x itself.
-    norm: "layer" or "rms".  Columns at or behind ``lengths[b]`` (int64 ``[B]``) are not read and come out as zero."""
+    norm: "layer" or "rms".  Columns at or behind ``lengths[b]`` (int64 ``[B]``) enter no result and come out as
+    zero; padding, and the gate of an item without columns, may hold anything."""
     _check(x, y, gate, scale, post, pre, norm, eps, lengths)
     w_post, b_post = post or (None, None)
     w_pre, b_pre = pre or (None, None)

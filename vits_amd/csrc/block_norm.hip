@@ -233,12 +233,13 @@ struct Spot {
     }
 };
 
-// The per-channel numbers of a pass in LDS: ones and zeros where something is not given.
+// The per-channel numbers of a pass in LDS: ones and zeros where something is not given.  An item without live columns has
+// no part in any sum, so its gate does not either: a NaN there (a mean over no columns) times its zeros would.
 enum { P_SCALE, P_GATE, P_WPOST, P_BPOST, P_WPRE, P_BPRE, P_COUNT };
 template <typename T>
-__device__ __forceinline__ void stage_params(float* par, const vk_block_norm_args& a, int b)
+__device__ __forceinline__ void stage_params(float* par, const vk_block_norm_args& a, int b, int live)
 {
-    const bool item = a.gate && a.gate_per_item;
+    const bool item = a.gate && a.gate_per_item && live > 0;
     const float* src[P_COUNT] = {a.scale, nullptr, a.w_post, a.b_post, a.w_pre, a.b_pre};
     for (int c = (int)threadIdx.x; c < a.channels; c += (int)blockDim.x) {
 #pragma unroll
@@ -265,7 +266,7 @@ void block_norm_kernel(NDev p)
     u32x4 xr[R], yr[R];
     if (a.y) at.load(yr, a.y, a.y_bstride, a.y_cstride);
     at.load(xr, a.x, a.x_bstride, a.x_cstride);
-    stage_params<T>(par, a, at.b);
+    stage_params<T>(par, a, at.b, at.live);
     __syncthreads();
     float h[R][E];
     if (a.y) {
@@ -341,7 +342,7 @@ void block_norm_backward_kernel(NDev p)
         u32x4 hr[R], dr[R];
         at.load(hr, a.h, a.h_bstride, a.h_cstride);
         at.load(dr, a.dn, a.dn_bstride, a.dn_cstride);
-        stage_params<T>(par, a, at.b);
+        stage_params<T>(par, a, at.b, at.live);
         __syncthreads();
         float mean[E], rstd[E], m1[E], m2[E];
         column_stats<LT, E, NW, R>([&](int r, float (&v)[E]) { unpack(v, hr[r]); keep_packed(hr[r]); }, at.rows, C, a.eps, layer, red, mean, rstd);
@@ -379,7 +380,7 @@ void block_norm_backward_kernel(NDev p)
             for (int e = 0; e < E; ++e) g[r][e] = (fmaf(d[e], w, -m1[e]) - (v[e] - mean[e]) * rstd[e] * m2[e]) * rstd[e];
         }
     } else {
-        stage_params<T>(par, a, at.b);
+        stage_params<T>(par, a, at.b, at.live);
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < R; ++r)
