@@ -364,7 +364,7 @@ int vk_expand_prior(const float* durations, const float* m, const float* logs, f
 /* ---- transformer blocks: attention with a bucketed relative position bias, norms around a block ----
  * Inference and training, element type `dtype` (VK_DTYPE_F32: exact fp32 matrix instruction;
  * VK_DTYPE_BF16: bf16 matrix inputs, fp32 accumulation and softmax).  Tensors are channel-major views
- * [batch, channels, time] with dense time, as everywhere here; strides count elements.  Batches are
+ * [batch, channels, time] with dense time, as everywhere here; strides count elements, 0..2^40.  Batches are
  * padded: `*_lengths[b]` (clamped to the tensor's length; NULL: full) says how far item b goes.  What lies behind it,
  * within the tensor, may be read but enters no result.
  *

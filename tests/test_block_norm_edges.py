@@ -58,3 +58,16 @@ def test_forward_mode_is_refused():
             with pytest.raises(native.NativeError, match="forward"):
                 block_norm_backward(*args, **keep)
         assert torch.equal(block_norm(**d)[0], h)
+
+
+def test_c_entries_refuse_negative_and_endless_strides():
+    L = native.lib()
+    room = dict(workspace=4096, workspace_bytes=1 << 40)
+    F = lambda **kw: L.vk_block_norm(C.byref(_args(**kw)), None)
+    B = lambda **kw: L.vk_block_norm_backward(C.byref(_args(**kw, **room)), None)
+    for n in ("x", "y", "gate", "h", "n"):
+        assert F(**{n + "_cstride": -100}) == -1 and F(**{n + "_bstride": -6400}) == -1, n
+        assert F(**{n + "_cstride": 1 << 61}) == -1, n
+    for n in ("y", "gate", "h", "dh", "dn", "dx", "dy", "dgate"):
+        assert B(**{n + "_cstride": -100}) == -1 and B(**{n + "_bstride": -6400}) == -1, n
+        assert B(**{n + "_cstride": 1 << 61}) == -1, n

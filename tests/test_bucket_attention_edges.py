@@ -259,3 +259,19 @@ def test_a_graph_outlives_the_buckets_it_was_captured_with():
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     del others
+
+
+# ---- C entries -------------------------------------------------------------------------------------
+
+def test_c_entries_refuse_negative_and_endless_strides():
+    L = native.lib()
+    names = [n + s for n in ("q", "k", "v", "out") for s in ("_bstride", "_cstride")]
+    more = [n + s for n in ("dout", "dq", "dk", "dv") for s in ("_bstride", "_cstride")]
+    room = dict(workspace=4096, workspace_bytes=1 << 40)
+    for n in names:
+        assert L.vk_bucket_attention(C.byref(_args(**{n: -100}, **room)), None) == -1, n
+    for n in names + more:
+        assert L.vk_bucket_attention_backward(C.byref(_args(**{n: -100}, **room)), None) == -1, n
+    for n in ("q", "out", "dout", "dq", "dk", "dv"):                           # a sum of them would wrap
+        assert L.vk_bucket_attention_backward(C.byref(_args(**{n + "_cstride": 1 << 62}, **room)), None) == -1, n
+        assert L.vk_bucket_attention_backward(C.byref(_args(**{n + "_bstride": 1 << 62}, **room)), None) == -1, n

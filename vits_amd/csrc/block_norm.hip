@@ -492,13 +492,14 @@ int fail(int code, const char* what, const char* msg)
 // Rows of one item are addressed with 32-bit offsets.
 bool item_fits(const void* p, int64_t cstride, const vk_block_norm_args* a)
 {
-    return !p || ((int64_t)(a->channels - 1) * (cstride < 0 ? -cstride : cstride) + a->length) * 4 < (int64_t)1 << 32;
+    return !p || ((int64_t)(a->channels - 1) * cstride + a->length) * 4 < (int64_t)1 << 32;
 }
+
+bool strides_ok(const void* p, int64_t bstride, int64_t cstride) { return !p || vk_strides_ok(bstride, cstride); }
 
 bool rows_apart(int64_t bstride, int64_t cstride, const vk_block_norm_args* a)
 {
-    if (a->channels > 1 && cstride < a->length) return false;
-    return a->batch <= 1 || bstride >= (int64_t)(a->channels - 1) * (a->channels > 1 ? cstride : 0) + a->length;
+    return vk_rows_apart(bstride, cstride, a->channels, a->length, a->batch);
 }
 
 int check(const vk_block_norm_args* a, const char* what, bool backward)
@@ -513,6 +514,12 @@ int check(const vk_block_norm_args* a, const char* what, bool backward)
     const bool some = a->batch > 0 && a->length > 0;
     if (some && !a->y && (a->gate || a->scale || a->w_post)) return fail(VK_E_ARG, what, "gate, scale and the norm after the block need y");
     if ((!a->w_post && a->b_post) || (!a->w_pre && a->b_pre)) return fail(VK_E_ARG, what, "a norm's bias needs its weight");
+    if (!strides_ok(a->x, a->x_bstride, a->x_cstride) || !strides_ok(a->y, a->y_bstride, a->y_cstride)
+        || !strides_ok(a->gate, a->gate_bstride, a->gate_cstride) || !strides_ok(a->h, a->h_bstride, a->h_cstride)
+        || !strides_ok(a->n, a->n_bstride, a->n_cstride) || !strides_ok(a->dh, a->dh_bstride, a->dh_cstride)
+        || !strides_ok(a->dn, a->dn_bstride, a->dn_cstride) || !strides_ok(a->dx, a->dx_bstride, a->dx_cstride)
+        || !strides_ok(a->dy, a->dy_bstride, a->dy_cstride) || !strides_ok(a->dgate, a->dgate_bstride, a->dgate_cstride))
+        return fail(VK_E_ARG, what, "a stride is negative or beyond 2^40");
     if (!item_fits(a->x, a->x_cstride, a) || !item_fits(a->y, a->y_cstride, a) || !item_fits(a->h, a->h_cstride, a)
         || !item_fits(a->n, a->n_cstride, a) || !item_fits(a->dh, a->dh_cstride, a) || !item_fits(a->dn, a->dn_cstride, a)
         || !item_fits(a->dx, a->dx_cstride, a) || !item_fits(a->dy, a->dy_cstride, a)

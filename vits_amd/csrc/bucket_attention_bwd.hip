@@ -550,9 +550,12 @@ extern "C" int vk_bucket_attention_backward(const vk_bucket_attention_args* a, v
     if (rows && (!a->out || !a->lse || !a->dout || !a->dq)) return vkba_fail(VK_E_ARG, what, "null out, lse, dout or dq");
     if (cols && (!a->dk || !a->dv)) return vkba_fail(VK_E_ARG, what, "null dk or dv");
     if (a->has_bias && !a->dbias) return vkba_fail(VK_E_ARG, what, "null dbias");
-    if (!vkba_rows_apart(a->dq_bstride, a->dq_cstride, (int64_t)a->heads * a->head_dim, a->queries, a->batch)
-        || !vkba_rows_apart(a->dk_bstride, a->dk_cstride, (int64_t)a->kv_heads * a->head_dim, a->keys, a->batch)
-        || !vkba_rows_apart(a->dv_bstride, a->dv_cstride, (int64_t)a->kv_heads * a->head_dim, a->keys, a->batch))
+    if (!vk_strides_ok(a->dout_bstride, a->dout_cstride) || !vk_strides_ok(a->dq_bstride, a->dq_cstride)
+        || !vk_strides_ok(a->dk_bstride, a->dk_cstride) || !vk_strides_ok(a->dv_bstride, a->dv_cstride))
+        return vkba_fail(VK_E_ARG, what, "a stride of dout, dq, dk or dv is negative or beyond 2^40");
+    if (!vk_rows_apart(a->dq_bstride, a->dq_cstride, (int64_t)a->heads * a->head_dim, a->queries, a->batch)
+        || !vk_rows_apart(a->dk_bstride, a->dk_cstride, (int64_t)a->kv_heads * a->head_dim, a->keys, a->batch)
+        || !vk_rows_apart(a->dv_bstride, a->dv_cstride, (int64_t)a->kv_heads * a->head_dim, a->keys, a->batch))
         return vkba_fail(VK_E_ARG, what, "rows of a gradient overlap");
     const int64_t need = workspace_floats(a) * 4;
     if (need > 0 && (!a->workspace || a->workspace_bytes < need))

@@ -380,7 +380,7 @@ extern "C" int vk_bucket_attention(const vk_bucket_attention_args* a, void* stre
     if (rc != VK_OK) return rc;
     if (a->batch == 0 || a->queries == 0) return VK_OK;
     if (!a->out || !a->lse) return vk_fail(VK_E_ARG, "vk_bucket_attention: null output");
-    if (!vkba_rows_apart(a->out_bstride, a->out_cstride, (int64_t)a->heads * a->head_dim, a->queries, a->batch))
+    if (!vk_rows_apart(a->out_bstride, a->out_cstride, (int64_t)a->heads * a->head_dim, a->queries, a->batch))
         return vk_fail(VK_E_ARG, "vk_bucket_attention: rows of out overlap");
     plan_forward(a, d, kw);
     const int64_t need = d.splits > 1 ? (int64_t)d.splits * a->batch * a->heads * a->queries * (a->head_dim + 2) * 4 : 0;

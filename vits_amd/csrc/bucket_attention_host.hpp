@@ -15,13 +15,6 @@ inline int vkba_fail(int code, const char* what, const char* msg)
     return vk_fail(code, buf);
 }
 
-// Views a pass writes: rows must not overlap.
-inline bool vkba_rows_apart(int64_t bstride, int64_t cstride, int64_t channels, int64_t length, int64_t batch)
-{
-    if (channels > 1 && cstride < length) return false;
-    return batch <= 1 || bstride >= (channels - 1) * (channels > 1 ? cstride : 0) + length;
-}
-
 // Fills the device struct with everything that does not depend on the pass.  `pointers`: also check them
 // (the workspace queries look at the sizes only).
 inline int vkba_check(const vk_bucket_attention_args* a, vkba::Dev& d, const char* what, bool pointers)
@@ -41,6 +34,9 @@ inline int vkba_check(const vk_bucket_attention_args* a, vkba::Dev& d, const cha
         if (a->has_bias && (!a->bias || !a->bucket_of)) return vkba_fail(VK_E_ARG, what, "null bias or bucket table");
         if (a->batch && a->queries && !a->q) return vkba_fail(VK_E_ARG, what, "null queries");
         if (a->batch && a->keys && (!a->k || !a->v)) return vkba_fail(VK_E_ARG, what, "null keys or values");
+        if (!vk_strides_ok(a->q_bstride, a->q_cstride) || !vk_strides_ok(a->k_bstride, a->k_cstride)
+            || !vk_strides_ok(a->v_bstride, a->v_cstride) || !vk_strides_ok(a->out_bstride, a->out_cstride))
+            return vkba_fail(VK_E_ARG, what, "a stride of q, k, v or out is negative or beyond 2^40");
     }
     memset(&d, 0, sizeof(d));
     d.q = a->q; d.qb = a->q_bstride; d.qc = a->q_cstride;
