@@ -71,3 +71,12 @@ def test_c_entries_refuse_negative_and_endless_strides():
     for n in ("y", "gate", "h", "dh", "dn", "dx", "dy", "dgate"):
         assert B(**{n + "_cstride": -100}) == -1 and B(**{n + "_bstride": -6400}) == -1, n
         assert B(**{n + "_cstride": 1 << 61}) == -1, n
+
+
+def test_the_workspace_query_refuses_what_the_pass_refuses():
+    L = native.lib()
+    for bad, code in ((dict(length=(1 << 31) - 1), -2), (dict(length=(1 << 28) + 1), -2), (dict(dtype=7), -2), (dict(channels=4097), -2),
+                      (dict(batch=-1), -1)):
+        a = _args(**bad)
+        assert L.vk_block_norm_backward_workspace_bytes(C.byref(a)) == code, bad
+        assert L.vk_block_norm_backward(C.byref(a), None) == code, bad

@@ -502,14 +502,22 @@ bool rows_apart(int64_t bstride, int64_t cstride, const vk_block_norm_args* a)
     return vk_rows_apart(bstride, cstride, a->channels, a->length, a->batch);
 }
 
-int check(const vk_block_norm_args* a, const char* what, bool backward)
+// What a workspace depends on.
+int check_sizes(const vk_block_norm_args* a, const char* what)
 {
     if (!a) return fail(VK_E_ARG, what, "null argument struct");
     if (a->batch < 0 || a->channels <= 0 || a->length < 0) return fail(VK_E_ARG, what, "bad size");
     if (a->dtype != VK_DTYPE_F32 && a->dtype != VK_DTYPE_BF16) return fail(VK_E_UNSUPPORTED, what, "dtype must be VK_DTYPE_F32 or VK_DTYPE_BF16");
-    if (a->norm != VK_NORM_LAYER && a->norm != VK_NORM_RMS) return fail(VK_E_ARG, what, "norm must be VK_NORM_LAYER or VK_NORM_RMS");
     if (a->channels > VK_BLOCK_NORM_MAX_CHANNELS) return fail(VK_E_UNSUPPORTED, what, "more than VK_BLOCK_NORM_MAX_CHANNELS channels");
     if (a->length > (1 << 28)) return fail(VK_E_UNSUPPORTED, what, "length beyond 2^28");
+    return VK_OK;
+}
+
+int check(const vk_block_norm_args* a, const char* what, bool backward)
+{
+    const int rc = check_sizes(a, what);
+    if (rc != VK_OK) return rc;
+    if (a->norm != VK_NORM_LAYER && a->norm != VK_NORM_RMS) return fail(VK_E_ARG, what, "norm must be VK_NORM_LAYER or VK_NORM_RMS");
     if (!(a->eps > 0.0f && a->eps < 1e30f)) return fail(VK_E_ARG, what, "eps must be positive and finite");
     const bool some = a->batch > 0 && a->length > 0;
     if (some && !a->y && (a->gate || a->scale || a->w_post)) return fail(VK_E_ARG, what, "gate, scale and the norm after the block need y");
@@ -631,9 +639,8 @@ extern "C" int vk_block_norm(const vk_block_norm_args* a, void* stream)
 
 extern "C" int64_t vk_block_norm_backward_workspace_bytes(const vk_block_norm_args* a)
 {
-    if (!a || a->batch < 0 || a->channels <= 0 || a->length < 0 || a->channels > VK_BLOCK_NORM_MAX_CHANNELS)
-        return fail(VK_E_ARG, "vk_block_norm_backward_workspace_bytes", "bad size");
-    return workspace_floats(a) * 4;
+    const int rc = check_sizes(a, "vk_block_norm_backward_workspace_bytes");
+    return rc != VK_OK ? rc : workspace_floats(a) * 4;
 }
 
 extern "C" int vk_block_norm_backward(const vk_block_norm_args* a, void* stream)
