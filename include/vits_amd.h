@@ -431,7 +431,8 @@ int vk_bucket_attention_backward(const vk_bucket_attention_args* a, void* stream
  * vk_block_norm_backward: dh, dn (either may be NULL: zero) -> dx, dy, dgate and the parameters' gradients (each may
  * be NULL if not wanted, but dx and, with y, dy), from h as stored, y, gate and the parameters:
  *     g = dh + N'(dn * w_pre)   dx = g   dgate = g * scale * z   dscale = sum g * gate * z   dy = N'(g * scale * gate * w_post)
- * The sums over columns are taken per workgroup and then over the workgroups in a fixed order, through `workspace`.  */
+ * The sums over columns are taken per workgroup and then over the workgroups in a fixed order, through `workspace`.
+ * With gate_per_item and dgate, batch <= 65530.  */
 #define VK_NORM_LAYER 0
 #define VK_NORM_RMS   1
 #define VK_BLOCK_NORM_MAX_CHANNELS 4096

@@ -152,7 +152,7 @@ def block_norm_backward(dh, dn, h, y=None, *, post=None, gate=None, scale=None, 
                         lengths=None) -> BlockNormGrads:
     """Gradients of ``block_norm`` for the gradients dh, dn of its outputs (either may be None), from the h it gave (x where
     there was no y) and what it took.  Sums over columns have a fixed order: the same inputs give the same bits.  Without
-    dn there is no gradient of ``pre``."""
+    dn there is no gradient of ``pre``.  With a gate ``[B, C, 1]`` and T > 1, B is at most 65530."""
     if dh is None and dn is None:
         raise ValueError("no gradient came in")
     if dn is not None and pre is None:

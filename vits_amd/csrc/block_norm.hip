@@ -10,8 +10,8 @@
 // channels are spread over the other lanes and the waves; column sums meet through LDS.
 // Bound by memory: forward reads x, y, gate and writes h, n; backward reads dh, dn, h, y, gate, writes dx, dy, dgate.
 // fp32, 32 x 256 x 2048: 75 us (4.5 TB/s), backward 136 us (3.9 TB/s).  bf16, 8 x 1024 x 4096, gate per item: 93 us (2.9 TB/s);
-// 8 x up to 2047 x 1024 backward 131 us (1.6 TB/s): that many channels leave one workgroup per CU, whose loads and
-// arithmetic alternate.
+// 8 x up to 2047 x 1024 backward 130 us (1.6 TB/s): that many channels leave one workgroup per CU, whose loads and
+// arithmetic alternate (and spill: 16 to 18 registers with eight rows per thread).
 #include <hip/hip_runtime.h>
 #include <atomic>
 #include <stdint.h>

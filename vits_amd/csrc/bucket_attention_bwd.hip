@@ -3,7 +3,7 @@
 // walks over keys), once for the gradients of the keys and values (a workgroup owns keys and walks
 // over the queries of every head that shares them).  Two walks cost 7 products instead of 5, but every
 // sum has one owner and a fixed order: no atomics, bit-identical from run to run.
-// Measured: 2 x 4095 causal positions, 16 bf16 heads of 128 on 4, 806 us (427 TFLOP/s of the formula's products), bound by
+// Measured: 2 x 4095 causal positions, 16 bf16 heads of 128 on 4, 802 us (428 TFLOP/s of the formula's products), bound by
 // matrix and vector instructions of two waves per SIMD that overlap little; 16 x up to 697, 2 fp32 heads of 96, 183 us.
 #include "bucket_attention.hpp"
 #include "api_internal.hpp"
@@ -21,9 +21,11 @@ struct Shape {
     static constexpr bool BF = sizeof(T) == 2;
     static constexpr bool SPLIT = BF && DP > 96;
     static constexpr int MIN_WAVES = BF || DP <= 64 ? 2 : 1;
-    // the next tile is loaded into registers while the present one is computed, unless that makes the rest spill (bf16,
-    // 8 x 8 heads of 96, 2048 positions: 594 us with, 533 without; 16 heads of 128 on 4, 1024 positions: 131, 110; the
-    // 128-channel kernel with tiles of 32 has room) or, fp32, takes the second wave
+    // the next tile is loaded into registers while the present one is computed, unless that makes the rest spill too much
+    // (bf16, 8 x 8 heads of 96, 2048 positions: 594 us with, 533 without; 16 heads of 128 on 4, 1024 positions: 131, 110) or,
+    // fp32, takes the second wave.  With 128 channels and tiles of 32 dq spills 21 registers with it, 4 without, and it pays
+    // all the same where the walk is long (2 x 16 heads on 4, 4095 causal positions: 791 us with, 834 without; two-sided
+    // 1419, 1476; 8 x 1024: 425, 413).
     static constexpr bool AHEAD = BF ? DP <= 64 || (DP > 96 && KW == 1) : MIN_WAVES == 1;
     static constexpr int KT_DQ = BF && DP > 96 && KW == 1 ? 32 : 64, KT_DKV = KT_DQ;
     static constexpr int OWN = Tile<T, DP, 64>::BYTES;                  // image of 64 of the workgroup's own rows
@@ -476,7 +478,8 @@ int launch_both(Dev d, hipStream_t st)
     if (blocks > 0x7fffffff) return vkba_fail(VK_E_UNSUPPORTED, what, "too many workgroups");
     d.kv_blocks = (int)blocks;
     // causal: the first keys have the most queries.  Where all workgroups find a place at once (two on every CU),
-    // those of dv come in the other order, so that a CU gets a long and a short one
+    // those of dv come in the other order, so that a CU gets a long and a short one (heads of 128: 16 of 1000 positions 90 us
+    // without, 86 with; 8 of 2000: 140, 135; launches that leave CUs empty are the same)
     d.fold = d.causal && 2 * blocks <= 512;
     const size_t need = S::IMAGES + 2 * S::KT_DKV * 4 + vkba_table_bytes(d);
     int rc = vkba_launch<bucket_dkv_kernel<T, DP, KW>>(d, (S::SPLIT ? 2 : 1) * blocks + (d.bias ? d.heads : 0),

@@ -5,9 +5,11 @@
 // columns = queries), so a query is a lane: its maximum and sum are lane-local but for one exchange
 // between the two lane halves, and the probabilities are already the right operand of P V.
 //
-// Bound by the softmax's vector instructions in bf16 (4 x 8191 positions, 8 heads of 64: 728 us, 755 TFLOP/s; per 32 x 32
-// scores 256 cycles of matrix instructions against some 640 of vector instructions), in fp32 by the matrix instruction's
-// rate and unequal lengths (16 x up to 1001 positions, 2 heads of 96: 101 us, 59 TFLOP/s).
+// Bound in bf16 by matrix and vector instructions one after the other (4 x 8191 positions, 8 heads of 64: 718 us,
+// 765 TFLOP/s; per 32 x 32 scores 256 cycles of matrix and some 640 of vector instructions, 765 us if none overlap; 8192
+// positions, whose rows are aligned: 675 us), in fp32 by the matrix instruction's rate and unequal lengths (16 x up to 1001
+// positions, 2 heads of 96: 101 us, 59 TFLOP/s; all 1001 long: 122 us, 101 TFLOP/s).  Of the variants only fp32 with 128
+// channels spills registers (36).
 #include "bucket_attention.hpp"
 #include "bucket_attention_narrow.hpp"
 #include "api_internal.hpp"

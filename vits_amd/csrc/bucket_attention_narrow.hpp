@@ -11,7 +11,7 @@
 // The order of the keys in the score tiles is chosen so that a lane's scores are consecutive positions, the right
 // operand of P V without crossing lanes.  The next tile's keys are requested before the present one's softmax.
 // Bound by memory with one row tile: keys and values are read once (a token over 16 x up to 16384 positions, 16 heads of
-// 128 on 4, bf16: 91 to 100 us, 3.6 to 3.9 TB/s); a sentence of 43 positions takes 14 us, all of it latency.
+// 128 on 4, bf16: 94 us, 3.8 TB/s; 128 bf16 channels spill 10 registers); a sentence of 43 positions takes 14 us, all latency.
 #include "bucket_attention.hpp"
 
 namespace vkba {
