@@ -4,7 +4,7 @@
 int vk_fail(int code, const char* msg);
 
 // Strides of a view in elements: kernels add them up in unsigned and 64-bit numbers, so none may be negative, nor so large
-// (8 TiB of bf16 and more) that a sum wraps.
+// (2 TiB of bf16 and more) that a sum wraps.
 inline bool vk_strides_ok(int64_t bstride, int64_t cstride)
 {
     constexpr int64_t most = (int64_t)1 << 40;
