@@ -376,7 +376,7 @@ int vk_expand_prior(const float* durations, const float* m, const float* logs, f
  *     lse_i = log sum_j exp(s_ij)          out_i = sum_j exp(s_ij - lse_i) v_j
  * A query without keys, and one at or behind query_lengths[b], gets out = 0 and lse = -inf.
  * bias [heads, buckets] fp32, bucket_of int32 [2 * max_distance + 1] (entries are clamped to the
- * buckets); has_bias = 0: no bias.  A bias of -inf, or below -2.35e38 as a type's lowest value is, forbids its bucket:
+ * buckets); has_bias = 0: no bias.  A bias of -inf, or below -2.36e38 as a type's lowest value is, forbids its bucket:
  * such a pair is none, a row of nothing else is one without keys, and the bucket's gradient is 0.  lse [B, heads, queries] fp32, dense.  Launches with few workgroups
  * share the keys out and join the shares through `workspace` (vk_bucket_attention_workspace_bytes, 16-byte aligned;
  * contents irrelevant before and after; calls that may overlap in time need one each).  scale > 0, batch * heads < 2^23.

@@ -191,7 +191,7 @@ def bucket_attention(q, k, v, bias=None, buckets: RelativeBuckets | None = None,
     ``scale * q_i . k_j + bias[head, buckets.bucket_of(j - pos_i)]`` with ``pos_i = query_start[b] + i`` (0 + i without
     it), over j < key_lengths[b] and, with ``causal``, j <= pos_i.
 
-    bias: float32 ``[heads, buckets.num_buckets]``, or None (no position bias); -inf or a type's lowest value (below -2.35e38)
+    bias: float32 ``[heads, buckets.num_buckets]``, or None (no position bias); -inf or a type's lowest value (below -2.36e38)
     forbids a bucket, and a query that may see nothing else is one without a key.  key_lengths, query_lengths, query_start:
     int64 ``[B]`` on the device, or None.  scale: 1 / sqrt(D) unless given, positive.  Queries without a key and those at or behind
     query_lengths[b] come out as zero.  What lies behind a length enters no result, nor do keys that ``causal`` hides from all
